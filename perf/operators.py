@@ -295,9 +295,11 @@ def setup_plan(case, s, nodes):
 
 
 def setup_append(case, s, nodes):
+    from muyo_llm_b200 import _abi
+
     row = s["qkv"].shape[1]
     s["params"] = nodes.paged_append_params(setup_cache(case, s["pages"], nodes), case["tokens"], n_dims=case["rot"],
-                                            rope_mode={"half": "neox", "pairs": "normal"}[case["mode"]], stride_q=row, stride_k=row, stride_v=row)
+                                            rope_mode=_abi.ROPE_NEOX if case["mode"] == "half" else _abi.ROPE_NORMAL, stride_q=row, stride_k=row, stride_v=row)
 
 
 def setup_attend(case, s, nodes):
