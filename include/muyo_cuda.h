@@ -455,6 +455,129 @@ int muyo_p2p_output(MuyoP2PGroup* g, float** y);
 int muyo_p2p_check(MuyoP2PGroup* g);
 int muyo_p2p_destroy(MuyoP2PGroup* g);
 
+/* ---- paged key-value cache: one step of several requests ------------------------------------------
+ * No counterpart in the reference, which decodes one sequence over one contiguous cache: these entry
+ * points give a server that runs a batch of requests the same step over a cache of fixed-size pages.
+ * A step is one muyo_cuda_paged_plan, then per layer muyo_cuda_paged_rope_append and
+ * muyo_cuda_paged_attention_decode. Lengths, tables, slots and positions stay in device memory, so
+ * the whole step can be captured in a CUDA graph and replayed; shapes and pointers are fixed at capture.
+ *
+ * A pool (one for keys, one for values, of equal strides) holds num_pages pages of page_size slots.
+ * Element (page, kv head, slot, channel) is at page * page_stride + head * head_stride +
+ * slot * slot_stride + channel. Strides of 0 mean the packed order [page][kv_head][slot][channel]
+ * (all three or none are 0). Pools are 16-byte aligned and strides are multiples of 16 bytes. A slot's
+ * number is page * page_size + slot. An element of an F8 (e4m3) pool, or of any pool, stands for
+ * its value times k_scale or v_scale (0 is read as 1); what does not fit e4m3 is stored as +-448. */
+#define MUYO_KV_F8 2u /* e4m3, paged pools only */
+typedef struct MuyoPagedCache {
+    uint32_t heads, kv_heads, head_dim; /* head_dim 16, 32, 64 or 128; at most 16 query heads per KV head */
+    uint32_t page_size, num_pages;      /* page_size * num_pages at most INT32_MAX */
+    uint32_t kv_dtype;                  /* MUYO_KV_F32, MUYO_KV_F16 or MUYO_KV_F8 */
+    float k_scale, v_scale;
+    uint64_t page_stride, head_stride, slot_stride;
+} MuyoPagedCache;
+
+/* Block tables and slot maps from request lengths. Request i of `seqs` (at most 8192) holds
+ * cached_lens[i] tokens; new_lens[i] > 0 asks for that many more, 0 for none, and a negative value
+ * ends the request: its pages go back to the ring and its length becomes 0.
+ *   block_table   [seqs][table_stride]: page of keys [j * page_size, (j + 1) * page_size) in column j;
+ *                 the pages that this step adds are written behind those that the request has
+ *   free_ring     [num_pages]: the free pages are entries head .. tail - 1 (modulo num_pages), taken at
+ *                 the head in the requests' order; the pages of ended requests are put at the tail, for
+ *                 the calls that follow
+ *   state         {head, tail, -, -}: counters that only grow; state_out receives {head, tail, requests
+ *                 refused in this step, tokens asked for in this step}
+ *   seq_lens      [seqs]: lengths after the step
+ *   query_start   [seqs + 1]: first token of each request in the ragged batch (requests in order)
+ *   positions, slots [max_tokens]: of each new token; slot -1 and position 0 for tokens of a refused
+ *                 request and behind the last one
+ * A request that does not fit its table row, that the free pages do not suffice for, or whose tokens
+ * pass max_tokens is refused as a whole: its length stays and it gets no page. Pages are counted
+ * in order, so once they run out every later request that needs one is refused too.
+ * seq_lens may be cached_lens and state_out may be state (the step in place); other buffers must not
+ * overlap. With both apart, a repeated call gives the same result. Lengths outside
+ * [0, table_stride * page_size] are clamped, and no content of any buffer leads out of bounds. */
+typedef struct MuyoPagedPlanParams {
+    uint32_t seqs, page_size, num_pages;
+    uint32_t table_stride; /* pages of a table row */
+    uint32_t max_tokens;   /* may be 0 */
+} MuyoPagedPlanParams;
+int muyo_cuda_paged_plan(const MuyoPagedPlanParams* p, const int32_t* cached_lens, const int32_t* new_lens,
+                         int32_t* block_table, int32_t* free_ring, const int64_t* state, int32_t* seq_lens,
+                         int32_t* query_start, int32_t* positions, int32_t* slots, int64_t* state_out, void* stream);
+
+/* The rotation that MuyoRopeParams describes (n_dims, freq_base, freq_scale, ext_factor, attn_factor,
+ * corr_dims, has_ff; the other fields are not read) as a table in float64: radians per position of
+ * each of the n_dims / 2 pairs, then the factor on the rotated values - n_dims / 2 + 1 doubles. The
+ * angles are those of muyo_cuda_rope, linear in the position, with base^(-2j / n_dims) in place of
+ * theta_scale^j. freq_factors: [n_dims / 2] on the device if has_ff. Made once per model. */
+int muyo_cuda_rope_frequencies(const MuyoRopeParams* p, const float* freq_factors, double* table, void* stream);
+
+/* Rotary positions and cache append of a ragged batch. Token t (row t of q, k and v: [heads][head_dim]
+ * or [kv_heads][head_dim] F32, rows stride_* apart) is turned by positions[t] * frequency (float64
+ * angles, rotation in float64 rounded once, as muyo_cuda_kv_append): NEOX pairs channels
+ * (j, j + n_dims/2), NORMAL pairs (2j, 2j + 1), of the n_dims channels from n_offs; the others pass
+ * unchanged. The turned q goes to q_out (which may be q with the same stride), the turned k and the
+ * v, divided by their scales and rounded to the pool's type, to slot slots[t] of their pools. A token
+ * with a slot outside [0, num_pages * page_size) is left out: no q_out row, no pool is written.
+ * Slots of one call must differ from one another: of two tokens in one slot either may stay, channel
+ * by channel. q may be NULL (keys and values only). n_dims 0 turns nothing and reads no freqs. */
+typedef struct MuyoPagedAppendParams {
+    MuyoPagedCache cache;
+    uint32_t tokens;
+    uint32_t rope_mode, n_dims, n_offs; /* n_dims and n_offs even */
+    uint32_t stride_q, stride_k, stride_v, stride_q_out; /* 0 = packed rows; multiples of 4 (rows 16-byte aligned) */
+} MuyoPagedAppendParams;
+int muyo_cuda_paged_rope_append(const MuyoPagedAppendParams* p, const float* q, const float* k, const float* v,
+                                const int32_t* positions, const int32_t* slots, const double* freqs, float* q_out,
+                                void* k_pool, void* v_pool, void* stream);
+
+/* Attention of one new token per request over its pages: for request i, keys
+ * max(0, seq_lens[i] - window) .. seq_lens[i] - 1 (window 0: all), the new token's own key among them;
+ *   out[i][h] = sum_j softmax_j(scale * q[i][h] . k_j) v_j,  lse[i][h] = log sum_j exp(scale * q . k_j).
+ * q, out: [seqs] rows of [heads][head_dim] F32, stride_q / stride_out apart, 16-byte aligned; lse
+ * [seqs][heads] F32 or NULL. A request without keys gets zeros and an lse of -inf. Lengths are clamped
+ * to [0, table_stride * page_size]. Keys on a page outside [0, num_pages) are left out. What lies in
+ * slots outside the attended keys is not used, NaN and infinities among it; attended keys and
+ * values, and q, are finite. One call at a time may use a workspace; it may hold anything before. */
+typedef struct MuyoPagedAttentionParams {
+    MuyoPagedCache cache;
+    uint32_t seqs;
+    uint32_t table_stride; /* pages of a table row */
+    uint32_t window;
+    uint32_t stride_q, stride_out; /* 0 = packed rows */
+    float scale;
+} MuyoPagedAttentionParams;
+size_t muyo_cuda_paged_attention_workspace_size(const MuyoPagedAttentionParams* p);
+int muyo_cuda_paged_attention_decode(const MuyoPagedAttentionParams* p, const float* q, const void* k_pool,
+                                     const void* v_pool, const int32_t* block_table, const int32_t* seq_lens, float* out,
+                                     float* lse, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- log probabilities of given tokens -------------------------------------------------------------
+ * No counterpart in the reference. For each of `rows` rows of `vocab` F32 logits (rows `stride` apart),
+ * with p = softmax(logits / temperature):
+ *   logprob[r]  = log p[tokens[r]] (-inf for an id outside [0, vocab))
+ *   entropy[r]  = -sum p log p (nats; may be NULL)
+ *   rank[r]     = number of ids in front of tokens[r] by (logit descending, id ascending) (may be NULL;
+ *                 vocab for an id outside)
+ *   top_ids, top_logprobs [rows][top_k] = the first top_k ids of that order and their log p (top_k
+ *                 0..32, at most vocab; NULL with top_k 0). The tie rule is muyo_cuda_argmax's.
+ * The sum over the other tokens is kept apart from the largest's 1, so that log p of an almost certain
+ * token keeps its relative accuracy. -inf logits (masked ids) have log p -inf; a row of nothing else
+ * has log p -inf, entropy 0 and ids 0 .. top_k - 1. A row with a NaN or +inf gives NaN log
+ * probabilities and entropy; NaN logits do not enter top_ids, and places that no id is left for hold -1.
+ * logits are 4-byte aligned, in any stride. One call at a time may use a workspace. */
+typedef struct MuyoTokenLogprobsParams {
+    uint32_t rows, vocab;
+    uint32_t stride; /* 0 = vocab */
+    uint32_t top_k;
+    float temperature; /* > 0 */
+} MuyoTokenLogprobsParams;
+size_t muyo_cuda_token_logprobs_workspace_size(const MuyoTokenLogprobsParams* p);
+int muyo_cuda_token_logprobs(const MuyoTokenLogprobsParams* p, const float* logits, const int32_t* tokens, float* logprob,
+                             float* entropy, int32_t* rank, int32_t* top_ids, float* top_logprobs, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

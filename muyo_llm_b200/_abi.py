@@ -22,7 +22,7 @@ MATVEC_BIAS0, MATVEC_BIAS1, MATVEC_SCALE0, MATVEC_SCALE1 = 1, 2, 4, 8
 MATMUL_BIAS, MATMUL_ACCUMULATE, MATMUL_TCGEN05 = 1, 2, 4
 GLU_HALVES, GLU_SWAPPED, GLU_SPLIT = 0, 1, 2
 ROPE_NORMAL, ROPE_NEOX = 0, 2
-KV_F32, KV_F16 = 0, 1
+KV_F32, KV_F16, KV_F8 = 0, 1, 2  # KV_F8 (e4m3): paged pools only
 
 
 class MuyoError(RuntimeError):
@@ -94,6 +94,28 @@ class LayerWeights(C.Structure):
     _fields_ = [(n, VP) for n in ("attn_norm", "wqkv", "bqkv", "wo", "ffn_norm", "wgate", "wup", "wdown")]
 
 
+class PagedCache(C.Structure):
+    _fields_ = _fields("heads, kv_heads, head_dim, page_size, num_pages, kv_dtype") + \
+               _fields("k_scale, v_scale", F32) + _fields("page_stride, head_stride, slot_stride", C.c_uint64)
+
+
+class PagedPlanParams(C.Structure):
+    _fields_ = _fields("seqs, page_size, num_pages, table_stride, max_tokens")
+
+
+class PagedAppendParams(C.Structure):
+    _fields_ = [("cache", PagedCache)] + _fields("tokens, rope_mode, n_dims, n_offs, stride_q, stride_k, stride_v, "
+                                                 "stride_q_out")
+
+
+class PagedAttentionParams(C.Structure):
+    _fields_ = [("cache", PagedCache)] + _fields("seqs, table_stride, window, stride_q, stride_out") + [("scale", F32)]
+
+
+class TokenLogprobsParams(C.Structure):
+    _fields_ = _fields("rows, vocab, stride, top_k") + [("temperature", F32)]
+
+
 P = C.POINTER
 # name -> (restype, argtypes)
 SIGNATURES = {
@@ -141,6 +163,13 @@ SIGNATURES = {
     "muyo_model_set_sampler": (C.c_int, [VP, P(SamplerParams), VP]),
     "muyo_cuda_mat_mul_f16_workspace_size": (C.c_size_t, [P(MatMulParams)]),
     "muyo_cuda_mat_mul_f16": (C.c_int, [P(MatMulParams), VP, VP, VP, VP, VP, C.c_size_t, VP]),
+    "muyo_cuda_paged_plan": (C.c_int, [P(PagedPlanParams)] + [VP] * 11),
+    "muyo_cuda_rope_frequencies": (C.c_int, [P(RopeParams), VP, VP, VP]),
+    "muyo_cuda_paged_rope_append": (C.c_int, [P(PagedAppendParams)] + [VP] * 10),
+    "muyo_cuda_paged_attention_workspace_size": (C.c_size_t, [P(PagedAttentionParams)]),
+    "muyo_cuda_paged_attention_decode": (C.c_int, [P(PagedAttentionParams)] + [VP] * 8 + [C.c_size_t, VP]),
+    "muyo_cuda_token_logprobs_workspace_size": (C.c_size_t, [P(TokenLogprobsParams)]),
+    "muyo_cuda_token_logprobs": (C.c_int, [P(TokenLogprobsParams)] + [VP] * 8 + [C.c_size_t, VP]),
     "muyo_p2p_handle_bytes": (C.c_size_t, []),
     "muyo_p2p_create": (C.c_int, [C.c_int, C.c_int, U32, P(VP), VP]),
     "muyo_p2p_connect": (C.c_int, [VP, VP]),

@@ -111,6 +111,45 @@ def attention_params(heads: int, kv_heads: int, head_dim: int, max_seq: int, n_k
                                 1.0 / math.sqrt(head_dim) if scale is None else scale)
 
 
+def paged_cache_params(heads: int, kv_heads: int, head_dim: int, *, page_size: int, num_pages: int,
+                       kv_dtype: int = _abi.KV_F16, order: str = "hnd", k_scale: float = 0.0, v_scale: float = 0.0,
+                       page_stride: int = 0, head_stride: int = 0, slot_stride: int = 0) -> _abi.PagedCache:
+    """Pools in packed [page][kv_head][slot][channel] order ("hnd") or [page][slot][kv_head][channel] ("nhd"), or of
+    the given strides (elements)."""
+    if order not in ("hnd", "nhd"):
+        raise ValueError(f"order {order!r}: hnd or nhd")
+    if not (page_stride or head_stride or slot_stride):
+        page_stride = page_size * kv_heads * head_dim
+        head_stride, slot_stride = ((page_size * head_dim, head_dim) if order == "hnd" else
+                                    (head_dim, kv_heads * head_dim))
+    return _abi.PagedCache(heads, kv_heads, head_dim, page_size, num_pages, kv_dtype, k_scale, v_scale, page_stride,
+                           head_stride, slot_stride)
+
+
+def paged_plan_params(seqs: int, *, page_size: int, num_pages: int, table_stride: int,
+                      max_tokens: int) -> _abi.PagedPlanParams:
+    return _abi.PagedPlanParams(seqs, page_size, num_pages, table_stride, max_tokens)
+
+
+def paged_append_params(cache: _abi.PagedCache, tokens: int, *, n_dims: int | None = None, n_offs: int = 0,
+                        rope_mode: int = _abi.ROPE_NEOX, stride_q: int = 0, stride_k: int = 0, stride_v: int = 0,
+                        stride_q_out: int = 0) -> _abi.PagedAppendParams:
+    """n_dims None turns the whole head, 0 nothing."""
+    return _abi.PagedAppendParams(cache, tokens, rope_mode, cache.head_dim if n_dims is None else n_dims, n_offs, stride_q,
+                                  stride_k, stride_v, stride_q_out)
+
+
+def paged_attention_params(cache: _abi.PagedCache, seqs: int, *, table_stride: int, window: int = 0, stride_q: int = 0,
+                           stride_out: int = 0, scale: float | None = None) -> _abi.PagedAttentionParams:
+    return _abi.PagedAttentionParams(cache, seqs, table_stride, window, stride_q, stride_out,
+                                     1.0 / math.sqrt(cache.head_dim) if scale is None else scale)
+
+
+def token_logprobs_params(rows: int, vocab: int, *, stride: int = 0, top_k: int = 0,
+                          temperature: float = 1.0) -> _abi.TokenLogprobsParams:
+    return _abi.TokenLogprobsParams(rows, vocab, stride, top_k, temperature)
+
+
 # ---- ops ------------------------------------------------------------------------------------------
 
 def mat_vec_f16(p, a, b, d, fuse0=None, fuse1=None, stream=None):
@@ -173,3 +212,40 @@ def attention_decode(p, q, k_cache, v_cache, out, workspace, workspace_bytes: in
 def kv_append(p, rope_base: float, k, v, k_cache, v_cache, pos, stream=None):
     return _abi.call("muyo_cuda_kv_append", p, rope_base, _ptr(k), _ptr(v), _ptr(k_cache), _ptr(v_cache), _ptr(pos),
                      _stream(stream))
+
+
+def paged_plan(p, cached_lens, new_lens, block_table, free_ring, state, seq_lens, query_start, positions, slots,
+               state_out, stream=None):
+    return _abi.call("muyo_cuda_paged_plan", p, _ptr(cached_lens), _ptr(new_lens), _ptr(block_table), _ptr(free_ring),
+                     _ptr(state), _ptr(seq_lens), _ptr(query_start), _ptr(positions), _ptr(slots), _ptr(state_out),
+                     _stream(stream))
+
+
+def rope_frequencies(p, table, freq_factors=None, stream=None):
+    """table: float64 [p.n_dims / 2 + 1]; p from rope_params (its scaling fields set by the caller)."""
+    return _abi.call("muyo_cuda_rope_frequencies", p, _ptr(freq_factors), _ptr(table), _stream(stream))
+
+
+def paged_rope_append(p, q, k, v, positions, slots, freqs, q_out, k_pool, v_pool, stream=None):
+    return _abi.call("muyo_cuda_paged_rope_append", p, _ptr(q), _ptr(k), _ptr(v), _ptr(positions), _ptr(slots), _ptr(freqs),
+                     _ptr(q_out), _ptr(k_pool), _ptr(v_pool), _stream(stream))
+
+
+def paged_attention_workspace_size(p) -> int:
+    return int(_abi.lib().muyo_cuda_paged_attention_workspace_size(p))
+
+
+def paged_attention_decode(p, q, k_pool, v_pool, block_table, seq_lens, out, workspace, workspace_bytes: int, lse=None,
+                           stream=None):
+    return _abi.call("muyo_cuda_paged_attention_decode", p, _ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(block_table),
+                     _ptr(seq_lens), _ptr(out), _ptr(lse), _ptr(workspace), workspace_bytes, _stream(stream))
+
+
+def token_logprobs_workspace_size(p) -> int:
+    return int(_abi.lib().muyo_cuda_token_logprobs_workspace_size(p))
+
+
+def token_logprobs(p, logits, tokens, logprob, workspace, workspace_bytes: int, entropy=None, rank=None, top_ids=None,
+                   top_logprobs=None, stream=None):
+    return _abi.call("muyo_cuda_token_logprobs", p, _ptr(logits), _ptr(tokens), _ptr(logprob), _ptr(entropy), _ptr(rank),
+                     _ptr(top_ids), _ptr(top_logprobs), _ptr(workspace), workspace_bytes, _stream(stream))
