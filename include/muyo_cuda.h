@@ -499,7 +499,7 @@ typedef struct MuyoPagedCache {
  * [0, table_stride * page_size] are clamped, and no content of any buffer leads out of bounds. */
 typedef struct MuyoPagedPlanParams {
     uint32_t seqs, page_size, num_pages;
-    uint32_t table_stride; /* pages of a table row */
+    uint32_t table_stride; /* pages of a table row; table_stride * page_size at most 2^30 */
     uint32_t max_tokens;   /* may be 0 */
 } MuyoPagedPlanParams;
 int muyo_cuda_paged_plan(const MuyoPagedPlanParams* p, const int32_t* cached_lens, const int32_t* new_lens,
@@ -543,7 +543,7 @@ int muyo_cuda_paged_rope_append(const MuyoPagedAppendParams* p, const float* q, 
 typedef struct MuyoPagedAttentionParams {
     MuyoPagedCache cache;
     uint32_t seqs;
-    uint32_t table_stride; /* pages of a table row */
+    uint32_t table_stride; /* pages of a table row; table_stride * page_size at most 2^30 */
     uint32_t window;
     uint32_t stride_q, stride_out; /* 0 = packed rows */
     float scale;

@@ -309,8 +309,8 @@ extern "C" int muyo_cuda_paged_plan(const MuyoPagedPlanParams* p, const int32_t*
                  "paged_plan: page_size, num_pages and table_stride must be positive");
     MUYO_REQUIRE((uint64_t)p->page_size * p->num_pages <= (uint64_t)INT_MAX,
                  "paged_plan: %u pages of %u slots exceed INT32_MAX slots", p->num_pages, p->page_size);
-    MUYO_REQUIRE((uint64_t)p->page_size * p->table_stride <= (uint64_t)INT_MAX,
-                 "paged_plan: a row of %u pages of %u slots exceeds INT32_MAX slots", p->table_stride, p->page_size);
+    MUYO_REQUIRE((uint64_t)p->page_size * p->table_stride <= (uint64_t)1 << 30,
+                 "paged_plan: a row of %u pages of %u slots exceeds 2^30 slots", p->table_stride, p->page_size);
     MUYO_REQUIRE(p->max_tokens < (uint32_t)INT_MAX, "paged_plan: max_tokens %u is not below INT32_MAX", p->max_tokens);
     MUYO_REQUIRE(cached_lens && new_lens && block_table && free_ring && state && seq_lens && query_start && state_out,
                  "paged_plan: null buffer");

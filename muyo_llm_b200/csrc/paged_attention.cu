@@ -1,125 +1,870 @@
 // Attention of one new token per request over a paged key-value cache.
+//
+// o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m), s_j = scale q . k_j, with the running maximum and sum of
+// an online softmax. Every key and value is read once, for all query heads of its KV head, so the bound is
+// the cache's bytes: 2 * keys * kv_heads * head_dim * sizeof(element).
+//
+// Work. The keys of a (request, KV head) are cut into tiles of KT keys (8 KB of keys and values, fewer for
+// small heads); all tiles of the batch, in order, are dealt out evenly and contiguously to the warps of one
+// CTA per SM. The dealing is done on the device from seq_lens (a scan per CTA), so a captured graph stays
+// right when lengths change, and no length spread leaves SMs idle: one request over 131071 keys and 200
+// requests over 60 to 2048 keys both keep every warp busy to within one tile. A warp that holds the whole of a
+// segment (the tiles of one request and KV head) writes its output; pieces of segments cut by a warp's border
+// are joined in shared memory by the CTA, those cut by a CTA's border by a second kernel from at most two
+// partials per CTA (m, l, o).
+//
+// A warp copies its tiles with cp.async into a ring of its own (no block barriers) STAGES - 1 tiles ahead;
+// the page numbers are fetched one tile further ahead. Rows are swizzled by 16-byte chunks so that the
+// fragment reads below meet no bank conflicts at 128-byte rows and wider.
+//
+// Products. mma.sync tiles of 16 rows x 8 keys (scores) and 16 rows x 8 channels (values). With at most 8 query
+// heads per KV head the 16 rows are the heads' leading halves and, below them, their remainders: an F32
+// operand x is split into two F16 (x = hi + lo, 22 bits; TF32 for an F32 cache), so one instruction makes both
+// products and a lane adds its own rows g and g + 8 at the end. With 9 to 16 heads the two halves take an
+// instruction each. q is brought near 2^14 by a power of two per head and the weights are formed as
+// 2^(s - m + 15), so that neither half falls under F16's normal range. F16 and e4m3 caches enter exactly;
+// F32 ones are split like q (the product of the two remainders is dropped for 9 to 16 heads only). Each
+// tile's products start from zero and are added to the running sums in F32: the tensor core's own additions
+// truncate, and long chains of them would drift. The channels' order in the contraction is free, so a
+// lane reads 16 contiguous bytes of a key's row for four (two) steps, and the keys of a step
+// are paired so that the scores' layout is the weights'. tcgen05 would hold 128 rows per tile for the 8 or 16 that one
+// token has; at these sizes the mma.sync issue is far below the memory time.
 #include "paged.cuh"
 
 namespace muyo {
 
-constexpr int kPagedThreads = 256;
-constexpr int kPagedMaxGroup = 16;
+constexpr int kPagedWarps = 8;
+constexpr int kPagedThreads = 32 * kPagedWarps;
 
 struct PagedAttnDev {
     PagedDev c;
     int seqs, table_stride, window;
+    int page_shift;  // log2(page_size), or -1
     long long stride_q, stride_out;
     float scale;  // softmax scale * k_scale
 };
 
-template <typename KV>
-__device__ __forceinline__ float pool_value(KV v);
-template <>
-__device__ __forceinline__ float pool_value<float>(float v)
+struct PagedDesc {
+    int seq, kv_head, pieces, pad;
+};
+
+template <int T, int HD, bool WIDE>
+struct PagedTile {
+    static constexpr int ES = T == MUYO_KV_F32 ? 4 : T == MUYO_KV_F16 ? 2 : 1;
+    static constexpr int RB = HD * ES;        // bytes of a row
+    static constexpr int CPR = RB / 16;       // 16-byte chunks of a row
+    static constexpr int KSTEP = T == MUYO_KV_F32 ? 8 : 16;
+    static constexpr int KT = 4096 / RB > 64 ? 64 : 4096 / RB;  // keys of a tile
+    static constexpr int STAGES = WIDE ? 2 : 3;
+    static constexpr int TILE = KT * RB;      // bytes of a tile's keys (or values)
+    static constexpr int ROWS = WIDE ? 16 : 8;
+    static constexpr int PART = ROWS * (HD + 2);  // floats of a partial: o [ROWS][HD], m, l
+    static constexpr int CHB = RB / 4 < 16 ? RB / 4 : 16;  // bytes of a lane's K read
+    static constexpr int EPC = CHB / ES;
+    static constexpr int NCH = RB / (4 * CHB);
+    static constexpr int KPS = T == MUYO_KV_F32 ? 2 : 4;   // a lane's channels per k-step
+    static constexpr int NKS = NCH * EPC / KPS;            // k-steps of a row
+    static constexpr int VPL = HD / 8;                     // a lane's channels of a value row
+    static constexpr int VCHB = VPL * ES < 16 ? VPL * ES : 16;
+    static constexpr int VE = VCHB / ES;
+    static constexpr int NVC = VPL / VE;
+    static constexpr int RING = STAGES * 2 * TILE;
+    static_assert(KT % KSTEP == 0 && KT * CPR % 32 == 0, "tile shape");
+    static_assert(RING >= PART * 4, "a drained ring holds a partial");
+    static constexpr size_t SMEM = (size_t)kPagedWarps * (RING + PART * 4);
+    static_assert(SMEM >= kPagedThreads * 8, "the scan shares the rings");
+};
+
+template <int CPR>
+__device__ __forceinline__ int k_chunk(int row, int ch)
 {
-    return v;
-}
-template <>
-__device__ __forceinline__ float pool_value<__half>(__half v)
-{
-    return __half2float(v);
-}
-template <>
-__device__ __forceinline__ float pool_value<__nv_fp8_e4m3>(__nv_fp8_e4m3 v)
-{
-    return float(v);
+    return CPR >= 8 ? ch ^ ((row & 1) << 2) : ch;
 }
 
-// One CTA per (request, KV head): each warp takes every eighth key with an online softmax per query head
-// (lanes over the channels), and the warps' (m, l, o) are joined in shared memory.
-template <typename KV, int HD>
-__global__ void __launch_bounds__(kPagedThreads) k_paged_attention(PagedAttnDev p, const float* __restrict__ q,
-                                                                   const KV* __restrict__ k_pool, const KV* __restrict__ v_pool,
-                                                                   const int32_t* __restrict__ table,
-                                                                   const int32_t* __restrict__ seq_lens,
-                                                                   float* __restrict__ out, float* __restrict__ lse)
+template <int CPR>
+__device__ __forceinline__ int v_chunk(int row, int ch)
 {
-    constexpr int E = (HD + 31) / 32;  // channels per lane
-    __shared__ float s_m[8][kPagedMaxGroup], s_l[8][kPagedMaxGroup], s_o[8][HD];
+    return CPR >= 8 ? ch ^ (((row >> 1) & 3) << 1) : CPR == 4 ? ch ^ (((row >> 1) & 1) << 1) : ch;
+}
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+// 16 bytes, or 16 zero bytes when !valid.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool valid)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait()
+{
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ float ex2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi)
+{
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// (a, b) as F16 pairs: the leading halves and the remainders.
+__device__ __forceinline__ void split_half2(float a, float b, uint32_t& hi, uint32_t& lo)
+{
+    hi = pack_half2(a, b);
+    const float2 h = h2_to_f2(hi);
+    lo = pack_half2(a - h.x, b - h.y);
+}
+
+__device__ __forceinline__ uint32_t tf32_rna(float x)
+{
+    uint32_t r;
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
+    return r;
+}
+
+__device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo)
+{
+    hi = tf32_rna(x);
+    lo = tf32_rna(x - __uint_as_float(hi));
+}
+
+// Two e4m3 (the low 16 bits) as two F16, exactly.
+__device__ __forceinline__ uint32_t e4m3x2_half2(uint32_t v)
+{
+    uint32_t r;
+    asm("{.reg .b16 t; cvt.u16.u32 t, %1; cvt.rn.f16x2.e4m3x2 %0, t;}" : "=r"(r) : "r"(v));
+    return r;
+}
+
+template <int BYTES>
+struct Chunk {
+    uint32_t w[BYTES < 4 ? 1 : BYTES / 4];
+    __device__ __forceinline__ void load(uint32_t addr)
+    {
+        if constexpr (BYTES == 16)
+            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr));
+        else if constexpr (BYTES == 8)
+            asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
+        else if constexpr (BYTES == 4)
+            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(addr));
+        else
+            asm volatile("{.reg .u16 t; ld.shared.u16 t, [%1]; cvt.u32.u16 %0, t;}" : "=r"(w[0]) : "r"(addr));
+    }
+};
+
+// The keys that a request's token sees, in tiles: [t0, t1).
+template <int KT>
+struct PagedSpan {
+    int n, begin, t0, t1;
+    __device__ __forceinline__ PagedSpan() {}
+    __device__ __forceinline__ PagedSpan(const PagedAttnDev& p, int len)
+    {
+        n = min(max(len, 0), p.table_stride * p.c.page_size);
+        begin = p.window > 0 ? max(0, n - p.window) : 0;
+        t0 = begin / KT;
+        t1 = n > begin ? (n + KT - 1) / KT : t0;
+    }
+};
+
+// A tile of the batch: tile t of request s under KV head h.
+template <int KT>
+struct PagedCursor {
+    int s, h, t;
+    PagedSpan<KT> span;
+    // The next tile; the caller knows that there is one.
+    __device__ __forceinline__ bool next(const PagedAttnDev& p, const int32_t* lens)
+    {
+        if (++t < span.t1)
+            return false;
+        if (++h == p.c.kv_heads) {
+            h = 0;
+            do {
+                span = PagedSpan<KT>(p, __ldg(lens + ++s));
+            } while (span.t1 == span.t0);
+        }
+        t = span.t0;
+        return true;
+    }
+};
+
+// Joins pieces of one segment, partials of the layout o [ROWS][HD], m [ROWS], l [ROWS]: a row's m is the
+// reference of its weights in log2 units, l their sum. Result in place of the caller's choice.
+template <int HD, int ROWS, typename PieceAt, typename Emit>
+__device__ __forceinline__ void join_row(int r, int pieces, PieceAt piece, Emit emit)
+{
+    const int lane = threadIdx.x & 31;
+    float M = -INFINITY;
+    for (int i = lane; i < pieces; i += 32)
+        M = fmaxf(M, piece(i)[ROWS * HD + r]);
+    M = warp_max(M);
+    float L = 0.0f, o[(HD + 31) / 32];
+#pragma unroll
+    for (int e = 0; e < (HD + 31) / 32; ++e)
+        o[e] = 0.0f;
+    for (int i0 = 0; i0 < pieces; i0 += 32) {
+        float w = 0.0f, lw = 0.0f;  // lane i holds piece i0 + i's weight
+        if (i0 + lane < pieces) {
+            const float* q = piece(i0 + lane);
+            const float l = q[ROWS * HD + ROWS + r];
+            w = l > 0.0f ? ex2(q[ROWS * HD + r] - M) : 0.0f;
+            lw = l * w;
+        }
+        L += warp_sum(lw);
+        const int n = min(32, pieces - i0);
+#pragma unroll 8
+        for (int i = 0; i < n; ++i) {
+            const float wi = __shfl_sync(0xffffffffu, w, i);
+            const float* q = piece(i0 + i) + r * HD;
+#pragma unroll
+            for (int e = 0; e < (HD + 31) / 32; ++e)
+                if (HD % 32 == 0 || lane < HD)
+                    o[e] = fmaf(wi, q[lane + 32 * e], o[e]);
+        }
+    }
+    emit(M, L, o);
+}
+
+template <int HD>
+__device__ __forceinline__ void write_row(const PagedAttnDev& p, int s, int head, float M, float L,
+                                          const float (&o)[(HD + 31) / 32], float* out, float* lse)
+{
+    const int lane = threadIdx.x & 31;
+    const float inv = L > 0.0f ? __fdiv_rn(p.c.v_scale, L) : 0.0f;
+    float* dst = out + s * p.stride_out + (long long)head * HD;
+#pragma unroll
+    for (int e = 0; e < (HD + 31) / 32; ++e)
+        if (HD % 32 == 0 || lane < HD)
+            dst[lane + 32 * e] = o[e] * inv;
+    if (lse && lane == 0)
+        lse[(size_t)s * p.c.heads + head] = L > 0.0f ? (M + log2f(L)) * 0.693147180559945f : -INFINITY;
+}
+
+template <int T, int HD, bool WIDE>
+__global__ void __launch_bounds__(kPagedThreads, 1)
+k_paged_attention(PagedAttnDev p, const float* __restrict__ q, const char* __restrict__ k_pool,
+                  const char* __restrict__ v_pool, const int32_t* __restrict__ table, const int32_t* __restrict__ lens,
+                  float* __restrict__ out, float* __restrict__ lse, float* __restrict__ part, PagedDesc* __restrict__ descs)
+{
+    using C = PagedTile<T, HD, WIDE>;
+    constexpr int KT = C::KT, HR = WIDE ? 2 : 1;  // HR: heads of a lane
+    extern __shared__ __align__(128) char paged_smem[];
+    __shared__ unsigned long long s_mask[kPagedWarps][C::STAGES];
+    __shared__ int s_first[kPagedWarps], s_last[kPagedWarps];  // 0 none, 1 open at the end, 2 ends here
+    __shared__ int s_seg[kPagedWarps][4];                      // request and KV head of the first and the last piece
+    __shared__ int s_works[kPagedWarps];
+    __shared__ int s_open;                                     // tiles of the CTA's last segment behind its range
+    __shared__ long long s_warp[kPagedWarps];
     pdl_wait();
     pdl_trigger();
-    const int s = blockIdx.x, kvh = blockIdx.y, G = p.c.group;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int n = min(max(seq_lens[s], 0), p.table_stride * p.c.page_size);
-    const int begin = p.window > 0 ? max(0, n - p.window) : 0;
-    const float* qs = q + s * p.stride_q + (long long)kvh * G * HD;
-    float* os = out + s * p.stride_out + (long long)kvh * G * HD;
-    float qv[kPagedMaxGroup][E], o[kPagedMaxGroup][E], m[kPagedMaxGroup], l[kPagedMaxGroup];
-#pragma unroll
-    for (int g = 0; g < kPagedMaxGroup; ++g) {
-        m[g] = -INFINITY;
-        l[g] = 0.0f;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const int d = lane + 32 * e;
-            qv[g][e] = g < G && d < HD ? qs[g * HD + d] * p.scale : 0.0f;
-            o[g][e] = 0.0f;
-        }
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int g = lane >> 2, cq = lane & 3;
+
+    // The batch's tiles: scanned[i] of all requests up to the end of thread i's share.
+    long long* scanned = reinterpret_cast<long long*>(paged_smem);
+    const int per = (p.seqs + kPagedThreads - 1) / kPagedThreads;
+    long long mine = 0;
+    for (int s = tid * per; s < min(tid * per + per, p.seqs); ++s) {
+        const PagedSpan<KT> span(p, __ldg(lens + s));
+        mine += (long long)(span.t1 - span.t0) * p.c.kv_heads;
     }
-    for (int t = begin + warp; t < n; t += 8) {
-        const int page = table[(size_t)s * p.table_stride + t / p.c.page_size];
-        if (page < 0 || page >= p.c.num_pages)
+    long long incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o)
+            incl += y;
+    }
+    if (lane == 31)
+        s_warp[warp] = incl;
+    if (tid == 0)
+        s_open = 0;
+    __syncthreads();
+    long long total = 0;
+#pragma unroll
+    for (int w = 0; w < kPagedWarps; ++w) {
+        if (w < warp)
+            incl += s_warp[w];
+        total += s_warp[w];
+    }
+    scanned[tid] = incl;
+    // Requests without keys.
+    for (int s = blockIdx.x * kPagedWarps + warp; s < p.seqs; s += gridDim.x * kPagedWarps) {
+        const PagedSpan<KT> span(p, __ldg(lens + s));
+        if (span.t1 > span.t0)
             continue;
-        const long long row = page * p.c.page_stride + kvh * p.c.head_stride + (t % p.c.page_size) * p.c.slot_stride;
-        float k[E], v[E];
+        for (int d = lane; d < p.c.heads * HD; d += 32)
+            out[s * p.stride_out + d] = 0.0f;
+        if (lse)
+            for (int h = lane; h < p.c.heads; h += 32)
+                lse[(size_t)s * p.c.heads + h] = -INFINITY;
+    }
+    __syncthreads();
+    const int ctas = (int)min((long long)gridDim.x, (total + kPagedWarps - 1) / kPagedWarps);  // CTAs with work
+    if ((int)blockIdx.x >= ctas) {
+        if (tid == 0)
+            descs[blockIdx.x] = PagedDesc{0, 0, 0, 0};
+        return;
+    }
+    const long long workers = (long long)ctas * kPagedWarps, worker = (long long)blockIdx.x * kPagedWarps + warp;
+    const long long u0 = worker * total / workers, u1 = (worker + 1) * total / workers;
+    const long long cta_end = ((long long)blockIdx.x + 1) * kPagedWarps * total / workers;
+    int left = (int)(u1 - u0), ahead = left;  // tiles to work on, to copy
+    PagedCursor<KT> cur;
+    if (left > 0) {
+        int lo = 0, hi = kPagedThreads - 1;  // the first share that reaches past u0
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (scanned[mid] > u0)
+                hi = mid;
+            else
+                lo = mid + 1;
+        }
+        long long rest = u0 - (lo > 0 ? scanned[lo - 1] : 0);
+        cur.s = lo * per;
+        for (;;) {
+            cur.span = PagedSpan<KT>(p, __ldg(lens + cur.s));
+            const long long units = (long long)(cur.span.t1 - cur.span.t0) * p.c.kv_heads;
+            if (rest < units)
+                break;
+            rest -= units;
+            ++cur.s;
+        }
+        const int tiles = cur.span.t1 - cur.span.t0;
+        cur.h = (int)(rest / tiles);
+        cur.t = cur.span.t0 + (int)(rest % tiles);
+    }
+    __syncthreads();  // scanned is done with: the rings take its place
+
+    char* ring = paged_smem + (size_t)warp * C::RING;
+    const uint32_t ring_at = smem_addr(ring);
+    float* first_part = reinterpret_cast<float*>(paged_smem + (size_t)kPagedWarps * C::RING) + (size_t)warp * C::PART;
+
+    // ---- copies ----
+    PagedCursor<KT> load = cur;
+    int pages[(KT + 31) / 32];
+    auto look_up = [&]() {
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const int d = lane + 32 * e;
-            k[e] = d < HD ? pool_value<KV>(k_pool[row + d]) : 0.0f;
-            v[e] = d < HD ? pool_value<KV>(v_pool[row + d]) : 0.0f;
+        for (int i = 0; i < (KT + 31) / 32; ++i) {
+            const int key = load.t * KT + i * 32 + lane;
+            pages[i] = -1;
+            if ((KT % 32 == 0 || lane < KT) && key < load.span.n && key >= load.span.begin) {
+                const int at = p.page_shift >= 0 ? key >> p.page_shift : key / p.c.page_size;
+                pages[i] = __ldg(table + (size_t)load.s * p.table_stride + at);
+            }
+        }
+    };
+    auto issue = [&](int stage) {
+        if (ahead > 0) {
+            long long off[(KT + 31) / 32];
+            unsigned long long mask = 0;
+#pragma unroll
+            for (int i = 0; i < (KT + 31) / 32; ++i) {
+                const int key = load.t * KT + i * 32 + lane;
+                const int slot = p.page_shift >= 0 ? key & (p.c.page_size - 1) : key % p.c.page_size;
+                const bool ok = pages[i] >= 0 && pages[i] < p.c.num_pages;
+                off[i] = ok ? (pages[i] * p.c.page_stride + load.h * p.c.head_stride + slot * p.c.slot_stride) * C::ES : 0;
+                mask |= (unsigned long long)__ballot_sync(0xffffffffu, ok) << (32 * i);
+            }
+            if (lane == 0)
+                s_mask[warp][stage] = mask;
+            const uint32_t kd = ring_at + stage * 2 * C::TILE, vd = kd + C::TILE;
+#pragma unroll
+            for (int i = 0; i < KT * C::CPR / 32; ++i) {
+                const int row = (i * 32 + lane) / C::CPR, ch = (i * 32 + lane) % C::CPR;
+                const long long o = __shfl_sync(0xffffffffu, off[i * 32 / C::CPR / 32], row & 31) + ch * 16;
+                const bool ok = (mask >> row) & 1;
+                copy16(kd + row * C::RB + k_chunk<C::CPR>(row, ch) * 16, k_pool + (ok ? o : 0), ok);
+                copy16(vd + row * C::RB + v_chunk<C::CPR>(row, ch) * 16, v_pool + (ok ? o : 0), ok);
+            }
+            if (--ahead > 0) {
+                load.next(p, lens);
+                look_up();
+            }
+        }
+        copies_commit();
+    };
+
+    // ---- the segment at hand ----
+    constexpr int NQ = T == MUYO_KV_F32 ? C::NKS * 2 * HR : C::NKS * 4 * HR;
+    uint32_t qf[NQ];              // fragments (F32 cache: q itself)
+    float qs[HR], m[HR], l[HR];   // m: reference of the weights, the running maximum - 15
+    float o[C::VPL][2 * HR];
+    bool fresh = true;            // a segment begins with the next tile
+    bool whole = false;           // this warp has the segment from its first tile on
+    auto begin_segment = [&]() {
+        whole = cur.t == cur.span.t0;
+        const float* qrow = q + cur.s * p.stride_q + (long long)cur.h * p.c.group * HD;
+#pragma unroll
+        for (int r = 0; r < HR; ++r) {
+            const int head = g + 8 * r;
+            float v[C::NKS * C::KPS];
+            float most = 0.0f;
+#pragma unroll
+            for (int k = 0; k < C::NKS; ++k) {
+                constexpr int SPC = C::EPC / C::KPS;  // steps of a chunk
+                const int d = (4 * (k / SPC) + cq) * C::EPC + (k % SPC) * C::KPS;
+#pragma unroll
+                for (int e = 0; e < C::KPS; e += 2) {
+                    const float2 x = head < p.c.group ? __ldg(reinterpret_cast<const float2*>(qrow + head * HD + d + e))
+                                                      : make_float2(0.0f, 0.0f);
+                    v[k * C::KPS + e] = x.x;
+                    v[k * C::KPS + e + 1] = x.y;
+                    most = fmaxf(most, fmaxf(fabsf(x.x), fabsf(x.y)));
+                }
+            }
+            qs[r] = p.scale * 1.4426950408889634f;
+            if constexpr (T == MUYO_KV_F32) {
+#pragma unroll
+                for (int i = 0; i < C::NKS * 2; ++i)
+                    qf[i * HR + r] = __float_as_uint(v[i]);
+            } else {
+                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+                // the exponent of 2^14 / most, by the bits; 0 and what is not finite stay as they are
+                const int e = (int)((__float_as_uint(most) >> 23) & 255u);
+                const int up = most > 0.0f && e < 255 ? min(126, 127 + 14 - e) : 0;
+                const float by = __uint_as_float((unsigned)(127 + max(up, -126)) << 23);
+                qs[r] *= __uint_as_float((unsigned)(127 - max(up, -126)) << 23);
+#pragma unroll
+                for (int k = 0; k < C::NKS; ++k) {
+                    uint32_t h0, l0, h1, l1;
+                    split_half2(v[4 * k] * by, v[4 * k + 1] * by, h0, l0);
+                    split_half2(v[4 * k + 2] * by, v[4 * k + 3] * by, h1, l1);
+                    if constexpr (WIDE) {  // [k][hi | lo][4]: rows g, g + 8 of each
+                        qf[k * 8 + r] = h0, qf[k * 8 + 2 + r] = h1;
+                        qf[k * 8 + 4 + r] = l0, qf[k * 8 + 6 + r] = l1;
+                    } else {
+                        qf[k * 4] = h0, qf[k * 4 + 1] = l0, qf[k * 4 + 2] = h1, qf[k * 4 + 3] = l1;
+                    }
+                }
+            }
+            m[r] = -INFINITY;
+            l[r] = 0.0f;
         }
 #pragma unroll
-        for (int g = 0; g < kPagedMaxGroup; ++g) {
-            if (g < G) {
-                float x = 0.0f;
+        for (int n = 0; n < C::VPL; ++n)
 #pragma unroll
-                for (int e = 0; e < E; ++e)
-                    x = fmaf(qv[g][e], k[e], x);
-                x = warp_sum(x);
-                const float mn = fmaxf(m[g], x), a = expf(m[g] - mn), w = expf(x - mn);
-                m[g] = mn;
-                l[g] = fmaf(l[g], a, w);
+            for (int e = 0; e < 2 * HR; ++e)
+                o[n][e] = 0.0f;
+    };
+
+    auto tile = [&](int stage) {
+        const uint32_t ks = ring_at + stage * 2 * C::TILE, vs = ks + C::TILE;
+        const unsigned long long mask = s_mask[warp][stage];
+        // scores: s[j][2 r + e] is head g + 8 r, key 8 j + 2 cq + e
+        float s[KT / 8][2 * HR];
 #pragma unroll
-                for (int e = 0; e < E; ++e)
-                    o[g][e] = fmaf(o[g][e], a, w * v[e]);
+        for (int j = 0; j < KT / 8; ++j) {
+            float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            const int row = j * 8 + g;
+#pragma unroll
+            for (int i = 0; i < C::NCH; ++i) {
+                Chunk<C::CHB> ch;
+                const int byte = (4 * i + cq) * C::CHB;
+                ch.load(ks + row * C::RB + k_chunk<C::CPR>(row, byte >> 4) * 16 + (byte & 15));
+                constexpr int SPC = C::EPC / C::KPS;
+#pragma unroll
+                for (int j2 = 0; j2 < SPC; ++j2) {
+                    const int k = i * SPC + j2;
+                    if constexpr (T == MUYO_KV_F32) {
+                        uint32_t bh[2], bl[2], ah[4], al[4];
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            split_tf32(__uint_as_float(ch.w[2 * j2 + e]), bh[e], bl[e]);
+#pragma unroll
+                            for (int r = 0; r < HR; ++r)
+                                split_tf32(__uint_as_float(qf[(k * 2 + e) * HR + r]), ah[2 * e + r], al[2 * e + r]);
+                        }
+                        if constexpr (WIDE) {
+                            mma_tf32(acc, al, bh[0], bh[1]);
+                            mma_tf32(acc, ah, bl[0], bl[1]);
+                            mma_tf32(acc, ah, bh[0], bh[1]);
+                        } else {
+                            const uint32_t a[4] = {ah[0], al[0], ah[2], al[2]};
+                            mma_tf32(acc, a, bl[0], bl[1]);
+                            mma_tf32(acc, a, bh[0], bh[1]);
+                        }
+                    } else {
+                        uint32_t b0, b1;
+                        if constexpr (T == MUYO_KV_F16) {
+                            b0 = ch.w[2 * j2], b1 = ch.w[2 * j2 + 1];
+                        } else {
+                            b0 = e4m3x2_half2(ch.w[j2]), b1 = e4m3x2_half2(ch.w[j2] >> 16);
+                        }
+                        if constexpr (WIDE) {
+                            const uint32_t lo[4] = {qf[k * 8 + 4], qf[k * 8 + 5], qf[k * 8 + 6], qf[k * 8 + 7]};
+                            const uint32_t hi[4] = {qf[k * 8], qf[k * 8 + 1], qf[k * 8 + 2], qf[k * 8 + 3]};
+                            mma_f16(acc, lo, b0, b1);
+                            mma_f16(acc, hi, b0, b1);
+                        } else {
+                            const uint32_t a[4] = {qf[k * 4], qf[k * 4 + 1], qf[k * 4 + 2], qf[k * 4 + 3]};
+                            mma_f16(acc, a, b0, b1);
+                        }
+                    }
+                }
             }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                if constexpr (WIDE) {
+                    s[j][e] = acc[e] * qs[0];
+                    s[j][2 + e] = acc[2 + e] * qs[1];
+                } else {
+                    s[j][e] = (acc[e] + acc[2 + e]) * qs[0];
+                }
+            }
+        }
+        constexpr unsigned long long ALL = KT == 64 ? ~0ull : (1ull << (KT & 63)) - 1;
+        if (mask != ALL) {
+#pragma unroll
+            for (int j = 0; j < KT / 8; ++j)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    if (!((mask >> (8 * j + 2 * cq + e)) & 1)) {
+#pragma unroll
+                        for (int r = 0; r < HR; ++r)
+                            s[j][2 * r + e] = -INFINITY;
+                    }
+        }
+        float alpha[HR];
+#pragma unroll
+        for (int r = 0; r < HR; ++r) {
+            float most = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < KT / 8; ++j)
+                most = fmaxf(most, fmaxf(s[j][2 * r], s[j][2 * r + 1]));
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+            const float mn = fmaxf(m[r], most - 15.0f);
+            const float ref = mn == -INFINITY ? 0.0f : mn;  // nothing seen yet: every weight is 2^-inf
+            alpha[r] = ex2(m[r] - ref);
+            m[r] = mn;
+            float sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < KT / 8; ++j)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    s[j][2 * r + e] = ex2(s[j][2 * r + e] - ref);
+                    sum += s[j][2 * r + e];
+                }
+            l[r] = fmaf(l[r], alpha[r], sum);
+        }
+        // values: o[n] is channel (8 ic + 2 cq + e) VE + n % VE of chunk ic = n / VE
+        if constexpr (T == MUYO_KV_F32) {
+            uint32_t wh[KT / 8][4], wl[KT / 8][4];
+#pragma unroll
+            for (int j = 0; j < KT / 8; ++j)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int r = 0; r < HR; ++r)
+                        split_tf32(s[j][2 * r + e], wh[j][2 * e + r], wl[j][2 * e + r]);
+#pragma unroll
+            for (int ic = 0; ic < C::NVC; ++ic) {
+                Chunk<C::VCHB> v[KT / 8][2];
+                const int byte = (8 * ic + g) * C::VCHB;
+#pragma unroll
+                for (int j = 0; j < KT / 8; ++j)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int row = 8 * j + 2 * cq + e;
+                        v[j][e].load(vs + row * C::RB + v_chunk<C::CPR>(row, byte >> 4) * 16 + (byte & 15));
+                    }
+#pragma unroll
+                for (int n = 0; n < C::VE; ++n) {
+                    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int j = 0; j < KT / 8; ++j) {
+                        uint32_t bh[2], bl[2];
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            split_tf32(__uint_as_float(v[j][e].w[n]), bh[e], bl[e]);
+                        if constexpr (WIDE) {
+                            mma_tf32(acc, wl[j], bh[0], bh[1]);
+                            mma_tf32(acc, wh[j], bl[0], bl[1]);
+                            mma_tf32(acc, wh[j], bh[0], bh[1]);
+                        } else {
+                            const uint32_t a[4] = {wh[j][0], wl[j][0], wh[j][2], wl[j][2]};
+                            mma_tf32(acc, a, bl[0], bl[1]);
+                            mma_tf32(acc, a, bh[0], bh[1]);
+                        }
+                    }
+                    float(&on)[2 * HR] = o[ic * C::VE + n];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        if constexpr (WIDE) {
+                            on[e] = fmaf(on[e], alpha[0], acc[e]);
+                            on[2 + e] = fmaf(on[2 + e], alpha[1], acc[2 + e]);
+                        } else {
+                            on[e] = fmaf(on[e], alpha[0], acc[e] + acc[2 + e]);
+                        }
+                    }
+                }
+            }
+        } else {
+            uint32_t w[KT / 16][WIDE ? 8 : 4];
+#pragma unroll
+            for (int j = 0; j < KT / 16; ++j)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {  // keys 16 j + 8 h + 2 cq + {0, 1}
+                    if constexpr (WIDE) {
+#pragma unroll
+                        for (int r = 0; r < 2; ++r)
+                            split_half2(s[2 * j + h][2 * r], s[2 * j + h][2 * r + 1], w[j][2 * h + r], w[j][4 + 2 * h + r]);
+                    } else {
+                        split_half2(s[2 * j + h][0], s[2 * j + h][1], w[j][2 * h], w[j][2 * h + 1]);
+                    }
+                }
+#pragma unroll
+            for (int ic = 0; ic < C::NVC; ++ic) {
+                Chunk<C::VCHB> v[KT / 16][4];
+                const int byte = (8 * ic + g) * C::VCHB;
+#pragma unroll
+                for (int j = 0; j < KT / 16; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int row = 16 * j + 8 * (e >> 1) + 2 * cq + (e & 1);
+                        v[j][e].load(vs + row * C::RB + v_chunk<C::CPR>(row, byte >> 4) * 16 + (byte & 15));
+                    }
+#pragma unroll
+                for (int n = 0; n < C::VE; ++n) {
+                    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int j = 0; j < KT / 16; ++j) {
+                        uint32_t b[2];
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            if constexpr (T == MUYO_KV_F16) {
+                                b[h] = __byte_perm(v[j][2 * h].w[n >> 1], v[j][2 * h + 1].w[n >> 1], n & 1 ? 0x7632 : 0x5410);
+                            } else {  // bytes n of both keys
+                                b[h] = e4m3x2_half2(__byte_perm(v[j][2 * h].w[n >> 2], v[j][2 * h + 1].w[n >> 2],
+                                                                (n & 3) | ((n & 3) + 4) << 4));
+                            }
+                        }
+                        if constexpr (WIDE) {
+                            const uint32_t lo[4] = {w[j][4], w[j][5], w[j][6], w[j][7]};
+                            const uint32_t hi[4] = {w[j][0], w[j][1], w[j][2], w[j][3]};
+                            mma_f16(acc, lo, b[0], b[1]);
+                            mma_f16(acc, hi, b[0], b[1]);
+                        } else {
+                            const uint32_t a[4] = {w[j][0], w[j][1], w[j][2], w[j][3]};
+                            mma_f16(acc, a, b[0], b[1]);
+                        }
+                    }
+                    float(&on)[2 * HR] = o[ic * C::VE + n];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        if constexpr (WIDE) {
+                            on[e] = fmaf(on[e], alpha[0], acc[e]);
+                            on[2 + e] = fmaf(on[2 + e], alpha[1], acc[2 + e]);
+                        } else {
+                            on[e] = fmaf(on[e], alpha[0], acc[e] + acc[2 + e]);
+                        }
+                    }
+                }
+            }
+        }
+    };
+
+    // Writes the segment's result: to `out` when it is complete, else as a partial.
+    auto end_segment = [&](float* partial) {
+#pragma unroll
+        for (int r = 0; r < HR; ++r) {
+            const int head = g + 8 * r;
+            float L = l[r];
+            L += __shfl_xor_sync(0xffffffffu, L, 1);
+            L += __shfl_xor_sync(0xffffffffu, L, 2);
+            float* dst;
+            float by = 1.0f;
+            if (partial) {
+                dst = partial + head * HD;
+                if (cq == 0) {
+                    partial[C::ROWS * HD + head] = m[r];
+                    partial[C::ROWS * HD + C::ROWS + head] = L;
+                }
+            } else {
+                if (head >= p.c.group)
+                    continue;
+                const int h = cur.h * p.c.group + head;
+                dst = out + cur.s * p.stride_out + (long long)h * HD;
+                by = L > 0.0f ? __fdiv_rn(p.c.v_scale, L) : 0.0f;
+                if (lse && cq == 0)
+                    lse[(size_t)cur.s * p.c.heads + h] = L > 0.0f ? (m[r] + log2f(L)) * 0.693147180559945f : -INFINITY;
+            }
+#pragma unroll
+            for (int ic = 0; ic < C::NVC; ++ic)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int d = (8 * ic + 2 * cq + e) * C::VE;
+                    if constexpr (C::VE >= 4) {
+#pragma unroll
+                        for (int n = 0; n < C::VE; n += 4)
+                            *reinterpret_cast<float4*>(dst + d + n) =
+                                make_float4(o[ic * C::VE + n][2 * r + e] * by, o[ic * C::VE + n + 1][2 * r + e] * by,
+                                            o[ic * C::VE + n + 2][2 * r + e] * by, o[ic * C::VE + n + 3][2 * r + e] * by);
+                    } else {
+#pragma unroll
+                        for (int n = 0; n < C::VE; ++n)
+                            dst[d + n] = o[ic * C::VE + n][2 * r + e] * by;
+                    }
+                }
+        }
+    };
+
+    int first = 0, last = 0;  // this warp's open pieces
+    if (left > 0) {
+        look_up();
+#pragma unroll
+        for (int i = 0; i < C::STAGES - 1; ++i)
+            issue(i);
+        int stage = 0, into = C::STAGES - 1;
+        while (left > 0) {
+            issue(into);
+            if (fresh)
+                begin_segment();
+            copies_wait<C::STAGES - 1>();
+            __syncwarp();
+            tile(stage);
+            __syncwarp();  // every lane is done with the stage before it is filled again
+            stage = stage + 1 == C::STAGES ? 0 : stage + 1;
+            into = into + 1 == C::STAGES ? 0 : into + 1;
+            --left;
+            const bool ends = cur.t + 1 == cur.span.t1;
+            fresh = ends;
+            if (ends || left == 0) {
+                if (whole && ends) {
+                    end_segment(nullptr);
+                } else if (!whole) {
+                    first = ends ? 2 : 1;
+                    if (lane == 0)
+                        s_seg[warp][0] = cur.s, s_seg[warp][1] = cur.h;
+                    end_segment(first_part);
+                } else {  // begun here, open: the ring is drained
+                    last = 1;
+                    if (lane == 0)
+                        s_seg[warp][2] = cur.s, s_seg[warp][3] = cur.h;
+                    end_segment(reinterpret_cast<float*>(ring));
+                }
+            }
+            if (left > 0)
+                cur.next(p, lens);
+            else if (!ends && u1 == cta_end && lane == 0)
+                s_open = cur.span.t1 - cur.t - 1;
         }
     }
-#pragma unroll
-    for (int g = 0; g < kPagedMaxGroup; ++g) {
-        if (g < G) {
-            if (lane == 0) {
-                s_m[warp][g] = m[g];
-                s_l[warp][g] = l[g];
-            }
-#pragma unroll
-            for (int e = 0; e < E; ++e)
-                if (lane + 32 * e < HD)
-                    s_o[warp][lane + 32 * e] = o[g][e];
-            __syncthreads();
-            float M = -INFINITY;
-            for (int w = 0; w < 8; ++w)
-                M = fmaxf(M, s_m[w][g]);
-            float L = 0.0f;
-            for (int w = 0; w < 8; ++w)
-                L += s_l[w][g] > 0.0f ? s_l[w][g] * expf(s_m[w][g] - M) : 0.0f;
-            for (int d = threadIdx.x; d < HD; d += kPagedThreads) {
-                float O = 0.0f;
-                for (int w = 0; w < 8; ++w)
-                    O += s_l[w][g] > 0.0f ? s_o[w][d] * expf(s_m[w][g] - M) : 0.0f;
-                os[g * HD + d] = L > 0.0f ? O / L * p.c.v_scale : 0.0f;
-            }
-            if (lse && threadIdx.x == 0)
-                lse[(size_t)s * p.c.heads + kvh * G + g] = L > 0.0f ? M + logf(L) : -INFINITY;
-            __syncthreads();
-        }
+    if (lane == 0) {
+        s_first[warp] = first;
+        s_last[warp] = last;
+        s_works[warp] = u1 > u0;
     }
+    __syncthreads();
+
+    // ---- the CTA's join ----
+    // A group is a piece that begins here (or, in the first warp with work, comes in) and those that follow it. Warp w
+    // joins the group that begins with its last piece, the first warp with work the one that comes in as well.
+    auto piece_of = [&](int w, bool head) -> const float* {
+        return head ? reinterpret_cast<const float*>(paged_smem + (size_t)kPagedWarps * C::RING) + (size_t)w * C::PART
+                    : reinterpret_cast<const float*>(paged_smem + (size_t)w * C::RING);
+    };
+    auto join = [&](bool incoming) {
+        // pieces: the group's own, then the first pieces of the warps behind it that have work
+        int pieces = 1;
+        bool ended = incoming && s_first[warp] == 2;
+        unsigned members = 0;  // warps whose first piece belongs
+        for (int w = warp + 1; w < kPagedWarps && !ended; ++w) {
+            if (s_first[w]) {
+                members |= 1u << w;
+                ++pieces;
+                ended = s_first[w] == 2;
+            }
+        }
+        const int seq = s_seg[warp][incoming ? 0 : 2], kvh = s_seg[warp][incoming ? 1 : 3];
+        auto piece = [&](int i) -> const float* {
+            return i == 0 ? piece_of(warp, incoming) : piece_of(__fns(members, 0, i), true);
+        };
+        float* to = part + ((size_t)blockIdx.x * 2 + (incoming ? 0 : 1)) * C::PART;
+        const bool complete = ended && !incoming;
+        for (int r = 0; r < p.c.group; ++r)
+            join_row<HD, C::ROWS>(r, pieces, piece, [&](float M, float L, const float(&v)[(HD + 31) / 32]) {
+                if (complete) {
+                    write_row<HD>(p, seq, kvh * p.c.group + r, M, L, v, out, lse);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < (HD + 31) / 32; ++e)
+                        if (HD % 32 == 0 || lane < HD)
+                            to[r * HD + lane + 32 * e] = v[e];
+                    if (lane == 0) {
+                        to[C::ROWS * HD + r] = M;
+                        to[C::ROWS * HD + C::ROWS + r] = L;
+                    }
+                }
+            });
+        return !ended && !incoming;  // begun in this CTA and open behind it
+    };
+    bool open = false;
+    if (last)
+        open = join(false);
+    bool leads = first != 0;
+    for (int w = 0; w < warp; ++w)
+        leads = leads && !s_works[w];
+    if (leads)
+        join(true);
+    // At most one group begins here and stays open: its warp says who joins what.
+    const int any_open = __syncthreads_or(open);
+    if (open && lane == 0) {
+        const long long end = cta_end + s_open;  // behind the segment
+        auto from = [&](long long cta) { return cta * kPagedWarps * total / workers; };
+        long long at = (end - 1) * ctas / total;
+        while (from(at + 1) <= end - 1)
+            ++at;
+        while (from(at) > end - 1)
+            --at;
+        descs[blockIdx.x] = PagedDesc{s_seg[warp][2], s_seg[warp][3], (int)(at - blockIdx.x) + 1, 0};
+    }
+    if (!any_open && tid == 0)
+        descs[blockIdx.x] = PagedDesc{0, 0, 0, 0};
+}
+
+// Joins the segment that begins in CTA blockIdx.x of the kernel above and ends in another: its last partial and the
+// first ones of the CTAs behind it. A warp per query head.
+template <int HD, int ROWS>
+__global__ void __launch_bounds__(ROWS * 32) k_paged_join(PagedAttnDev p, const float* __restrict__ part,
+                                                          const PagedDesc* __restrict__ descs, float* __restrict__ out,
+                                                          float* __restrict__ lse)
+{
+    constexpr int PART = ROWS * (HD + 2);
+    pdl_wait();
+    pdl_trigger();
+    const PagedDesc d = descs[blockIdx.x];
+    const int r = threadIdx.x >> 5;
+    if (d.pieces == 0 || r >= p.c.group)
+        return;
+    const size_t at = blockIdx.x;
+    auto piece = [&](int i) -> const float* { return part + (i == 0 ? at * 2 + 1 : (at + i) * 2) * PART; };
+    join_row<HD, ROWS>(r, d.pieces, piece, [&](float M, float L, const float(&v)[(HD + 31) / 32]) {
+        write_row<HD>(p, d.seq, d.kv_head * p.c.group + r, M, L, v, out, lse);
+    });
 }
 
 static int paged_attention_prepare(const MuyoPagedAttentionParams* p, PagedAttnDev& d)
@@ -129,8 +874,8 @@ static int paged_attention_prepare(const MuyoPagedAttentionParams* p, PagedAttnD
     if (rc != MUYO_OK)
         return rc;
     MUYO_REQUIRE(p->seqs > 0 && p->seqs <= (uint32_t)INT_MAX, "paged_attention: seqs must be in [1, INT32_MAX]");
-    MUYO_REQUIRE(p->table_stride > 0 && (uint64_t)p->cache.page_size * p->table_stride <= (uint64_t)INT_MAX,
-                 "paged_attention: table_stride %u must be positive, and a row at most INT32_MAX slots", p->table_stride);
+    MUYO_REQUIRE(p->table_stride > 0 && (uint64_t)p->cache.page_size * p->table_stride <= (uint64_t)1 << 30,
+                 "paged_attention: table_stride %u must be positive, and a row at most 2^30 slots", p->table_stride);
     MUYO_REQUIRE(p->window <= (uint32_t)INT_MAX, "paged_attention: window %u exceeds INT32_MAX", p->window);
     MUYO_REQUIRE(std::isfinite(p->scale), "paged_attention: scale must be finite");
     const uint32_t row = p->cache.heads * p->cache.head_dim;
@@ -140,30 +885,60 @@ static int paged_attention_prepare(const MuyoPagedAttentionParams* p, PagedAttnD
     MUYO_REQUIRE((d.stride_q | d.stride_out) % 4 == 0, "paged_attention: row strides must be multiples of 4");
     d.seqs = (int)p->seqs, d.table_stride = (int)p->table_stride, d.window = (int)p->window;
     d.scale = p->scale * d.c.k_scale;
+    d.page_shift = -1;
+    for (int s = 0; s < 31; ++s)
+        if (d.c.page_size == 1 << s)
+            d.page_shift = s;
     return MUYO_OK;
 }
 
-template <typename KV, int HD>
-static int launch_paged_attention(const PagedAttnDev& d, const float* q, const void* k, const void* v, const int32_t* table,
-                                  const int32_t* lens, float* out, float* lse, void* stream)
+// CTAs: one per SM, fewer when the tables could not hold a tile per warp.
+static int paged_attention_ctas(const PagedAttnDev& d)
 {
-    MUYO_CUDA_TRY(launch_kernel(k_paged_attention<KV, HD>, dim3(d.seqs, d.c.kv_heads), dim3(kPagedThreads), 0,
-                                as_stream(stream), true, d, q, static_cast<const KV*>(k), static_cast<const KV*>(v), table,
-                                lens, out, lse));
+    const long long tiles = ((long long)d.table_stride * d.c.page_size + 7) / 8 * d.c.kv_heads;
+    const long long most = (tiles * d.seqs + kPagedWarps - 1) / kPagedWarps;
+    return (int)(most < sm_count() ? most : sm_count());
+}
+
+static size_t paged_attention_parts(const PagedAttnDev& d)
+{
+    return (size_t)paged_attention_ctas(d) * 2 * (d.c.group > 8 ? 16 : 8) * (d.c.head_dim + 2) * sizeof(float);
+}
+
+template <int T, int HD, bool WIDE>
+static int launch_paged_attention(const PagedAttnDev& d, const float* q, const void* k, const void* v, const int32_t* table,
+                                  const int32_t* lens, float* out, float* lse, void* ws, void* stream)
+{
+    using C = PagedTile<T, HD, WIDE>;
+    auto kernel = k_paged_attention<T, HD, WIDE>;
+    MUYO_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM));
+    const int ctas = paged_attention_ctas(d);
+    float* part = static_cast<float*>(ws);
+    PagedDesc* descs = reinterpret_cast<PagedDesc*>(static_cast<char*>(ws) + paged_attention_parts(d));
+    MUYO_CUDA_TRY(launch_kernel(kernel, dim3(ctas), dim3(kPagedThreads), C::SMEM, as_stream(stream), true, d, q,
+                                static_cast<const char*>(k), static_cast<const char*>(v), table, lens, out, lse, part, descs));
+    MUYO_LAUNCH_CHECK();
+    MUYO_CUDA_TRY(launch_kernel(k_paged_join<HD, C::ROWS>, dim3(ctas), dim3(C::ROWS * 32), 0, as_stream(stream), true, d,
+                                part, descs, out, lse));
     MUYO_LAUNCH_CHECK();
     return MUYO_OK;
 }
 
-template <typename KV>
+template <int T>
 static int launch_paged_attention_dim(const PagedAttnDev& d, const float* q, const void* k, const void* v,
-                                      const int32_t* table, const int32_t* lens, float* out, float* lse, void* stream)
+                                      const int32_t* table, const int32_t* lens, float* out, float* lse, void* ws,
+                                      void* stream)
 {
+#define MUYO_PAGED_DIM(HD)                                                                                      \
+    return d.c.group > 8 ? launch_paged_attention<T, HD, true>(d, q, k, v, table, lens, out, lse, ws, stream)   \
+                         : launch_paged_attention<T, HD, false>(d, q, k, v, table, lens, out, lse, ws, stream)
     switch (d.c.head_dim) {
-        case 16: return launch_paged_attention<KV, 16>(d, q, k, v, table, lens, out, lse, stream);
-        case 32: return launch_paged_attention<KV, 32>(d, q, k, v, table, lens, out, lse, stream);
-        case 64: return launch_paged_attention<KV, 64>(d, q, k, v, table, lens, out, lse, stream);
-        default: return launch_paged_attention<KV, 128>(d, q, k, v, table, lens, out, lse, stream);
+        case 16: MUYO_PAGED_DIM(16);
+        case 32: MUYO_PAGED_DIM(32);
+        case 64: MUYO_PAGED_DIM(64);
+        default: MUYO_PAGED_DIM(128);
     }
+#undef MUYO_PAGED_DIM
 }
 
 }  // namespace muyo
@@ -173,7 +948,9 @@ using namespace muyo;
 extern "C" size_t muyo_cuda_paged_attention_workspace_size(const MuyoPagedAttentionParams* p)
 {
     PagedAttnDev d{};
-    return p && paged_attention_prepare(p, d) == MUYO_OK ? 256 : 0;
+    if (!p || paged_attention_prepare(p, d) != MUYO_OK)
+        return 0;
+    return paged_attention_parts(d) + (size_t)paged_attention_ctas(d) * sizeof(PagedDesc);
 }
 
 extern "C" int muyo_cuda_paged_attention_decode(const MuyoPagedAttentionParams* p, const float* q, const void* k_pool,
@@ -195,10 +972,10 @@ extern "C" int muyo_cuda_paged_attention_decode(const MuyoPagedAttentionParams* 
     MUYO_REQUIRE(aligned16(workspace), "paged_attention: workspace must be 16-byte aligned");
     switch (p->cache.kv_dtype) {
         case MUYO_KV_F32:
-            return launch_paged_attention_dim<float>(d, q, k_pool, v_pool, block_table, seq_lens, out, lse, stream);
+            return launch_paged_attention_dim<MUYO_KV_F32>(d, q, k_pool, v_pool, block_table, seq_lens, out, lse, workspace, stream);
         case MUYO_KV_F16:
-            return launch_paged_attention_dim<__half>(d, q, k_pool, v_pool, block_table, seq_lens, out, lse, stream);
+            return launch_paged_attention_dim<MUYO_KV_F16>(d, q, k_pool, v_pool, block_table, seq_lens, out, lse, workspace, stream);
         default:
-            return launch_paged_attention_dim<__nv_fp8_e4m3>(d, q, k_pool, v_pool, block_table, seq_lens, out, lse, stream);
+            return launch_paged_attention_dim<MUYO_KV_F8>(d, q, k_pool, v_pool, block_table, seq_lens, out, lse, workspace, stream);
     }
 }
