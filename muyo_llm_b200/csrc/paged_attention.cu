@@ -209,8 +209,8 @@ struct PagedCursor {
     }
 };
 
-// Joins pieces of one segment, partials of the layout o [ROWS][HD], m [ROWS], l [ROWS]: a row's m is the
-// reference of its weights in log2 units, l their sum. Result in place of the caller's choice.
+// Joins one row of the pieces of a segment, partials of the layout o [ROWS][HD], m [ROWS], l [ROWS]: a row's m is
+// the reference of its weights in log2 units, l their sum. piece(i) is asked for by lane i % 32 only.
 template <int HD, int ROWS, typename PieceAt, typename Emit>
 __device__ __forceinline__ void join_row(int r, int pieces, PieceAt piece, Emit emit)
 {
@@ -225,10 +225,11 @@ __device__ __forceinline__ void join_row(int r, int pieces, PieceAt piece, Emit 
         o[e] = 0.0f;
     for (int i0 = 0; i0 < pieces; i0 += 32) {
         float w = 0.0f, lw = 0.0f;  // lane i holds piece i0 + i's weight
+        const float* at = nullptr;
         if (i0 + lane < pieces) {
-            const float* q = piece(i0 + lane);
-            const float l = q[ROWS * HD + ROWS + r];
-            w = l > 0.0f ? ex2(q[ROWS * HD + r] - M) : 0.0f;
+            at = piece(i0 + lane);
+            const float l = at[ROWS * HD + ROWS + r];
+            w = l > 0.0f ? ex2(at[ROWS * HD + r] - M) : 0.0f;
             lw = l * w;
         }
         L += warp_sum(lw);
@@ -236,11 +237,12 @@ __device__ __forceinline__ void join_row(int r, int pieces, PieceAt piece, Emit 
 #pragma unroll 8
         for (int i = 0; i < n; ++i) {
             const float wi = __shfl_sync(0xffffffffu, w, i);
-            const float* q = piece(i0 + i) + r * HD;
+            const float* row =
+                reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(at), i)) + r * HD;
 #pragma unroll
             for (int e = 0; e < (HD + 31) / 32; ++e)
                 if (HD % 32 == 0 || lane < HD)
-                    o[e] = fmaf(wi, q[lane + 32 * e], o[e]);
+                    o[e] = fmaf(wi, row[lane + 32 * e], o[e]);
         }
     }
     emit(M, L, o);
@@ -781,68 +783,68 @@ k_paged_attention(PagedAttnDev p, const float* __restrict__ q, const char* __res
     __syncthreads();
 
     // ---- the CTA's join ----
-    // A group is a piece that begins here (or, in the first warp with work, comes in) and those that follow it. Warp w
-    // joins the group that begins with its last piece, the first warp with work the one that comes in as well.
-    auto piece_of = [&](int w, bool head) -> const float* {
-        return head ? reinterpret_cast<const float*>(paged_smem + (size_t)kPagedWarps * C::RING) + (size_t)w * C::PART
-                    : reinterpret_cast<const float*>(paged_smem + (size_t)w * C::RING);
-    };
-    auto join = [&](bool incoming) {
-        // pieces: the group's own, then the first pieces of the warps behind it that have work
-        int pieces = 1;
-        bool ended = incoming && s_first[warp] == 2;
-        unsigned members = 0;  // warps whose first piece belongs
-        for (int w = warp + 1; w < kPagedWarps && !ended; ++w) {
-            if (s_first[w]) {
-                members |= 1u << w;
-                ++pieces;
-                ended = s_first[w] == 2;
+    // A group is a piece that begins here (or, in the first warp with work, comes in) and the first pieces of the warps
+    // behind it, up to the one where the segment ends. Every warp takes rows of every group.
+    bool came_in = true;  // no warp before w had work
+    bool described = false;
+    int turn = 0;
+    for (int w = 0; w < kPagedWarps; ++w) {
+        for (int kind = 0; kind < 2; ++kind) {
+            const bool incoming = kind == 0;
+            if (incoming ? !(came_in && s_first[w]) : !s_last[w])
+                continue;
+            bool ended = incoming && s_first[w] == 2;
+            int pieces = 1, from = w;  // from: the warp of this lane's piece
+            for (int v = w + 1; v < kPagedWarps && !ended; ++v) {
+                if (s_first[v]) {
+                    from = pieces == lane ? v : from;
+                    ++pieces;
+                    ended = s_first[v] == 2;
+                }
+            }
+            const int seq = s_seg[w][incoming ? 0 : 2], kvh = s_seg[w][incoming ? 1 : 3];
+            auto piece = [&](int i) -> const float* {
+                return reinterpret_cast<const float*>(
+                    incoming || i > 0 ? paged_smem + (size_t)kPagedWarps * C::RING + (size_t)from * C::PART * 4
+                                      : paged_smem + (size_t)from * C::RING);
+            };
+            float* to = part + ((size_t)blockIdx.x * 2 + (incoming ? 0 : 1)) * C::PART;
+            const bool complete = ended && !incoming;
+            for (int r = 0; r < p.c.group; ++r) {
+                if ((turn++ & (kPagedWarps - 1)) != warp)
+                    continue;
+                join_row<HD, C::ROWS>(r, pieces, piece, [&](float M, float L, const float(&v)[(HD + 31) / 32]) {
+                    if (complete) {
+                        write_row<HD>(p, seq, kvh * p.c.group + r, M, L, v, out, lse);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < (HD + 31) / 32; ++e)
+                            if (HD % 32 == 0 || lane < HD)
+                                to[r * HD + lane + 32 * e] = v[e];
+                        if (lane == 0) {
+                            to[C::ROWS * HD + r] = M;
+                            to[C::ROWS * HD + C::ROWS + r] = L;
+                        }
+                    }
+                });
+            }
+            if (!ended && !incoming) {  // begun in this CTA and open behind it (one group at most): who joins it
+                described = true;
+                if (tid == 0) {
+                    const long long end = cta_end + s_open;  // behind the segment
+                    auto begin = [&](long long cta) { return cta * kPagedWarps * total / workers; };
+                    long long at = (end - 1) * ctas / total;
+                    while (begin(at + 1) <= end - 1)
+                        ++at;
+                    while (begin(at) > end - 1)
+                        --at;
+                    descs[blockIdx.x] = PagedDesc{seq, kvh, (int)(at - blockIdx.x) + 1, 0};
+                }
             }
         }
-        const int seq = s_seg[warp][incoming ? 0 : 2], kvh = s_seg[warp][incoming ? 1 : 3];
-        auto piece = [&](int i) -> const float* {
-            return i == 0 ? piece_of(warp, incoming) : piece_of(__fns(members, 0, i), true);
-        };
-        float* to = part + ((size_t)blockIdx.x * 2 + (incoming ? 0 : 1)) * C::PART;
-        const bool complete = ended && !incoming;
-        for (int r = 0; r < p.c.group; ++r)
-            join_row<HD, C::ROWS>(r, pieces, piece, [&](float M, float L, const float(&v)[(HD + 31) / 32]) {
-                if (complete) {
-                    write_row<HD>(p, seq, kvh * p.c.group + r, M, L, v, out, lse);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < (HD + 31) / 32; ++e)
-                        if (HD % 32 == 0 || lane < HD)
-                            to[r * HD + lane + 32 * e] = v[e];
-                    if (lane == 0) {
-                        to[C::ROWS * HD + r] = M;
-                        to[C::ROWS * HD + C::ROWS + r] = L;
-                    }
-                }
-            });
-        return !ended && !incoming;  // begun in this CTA and open behind it
-    };
-    bool open = false;
-    if (last)
-        open = join(false);
-    bool leads = first != 0;
-    for (int w = 0; w < warp; ++w)
-        leads = leads && !s_works[w];
-    if (leads)
-        join(true);
-    // At most one group begins here and stays open: its warp says who joins what.
-    const int any_open = __syncthreads_or(open);
-    if (open && lane == 0) {
-        const long long end = cta_end + s_open;  // behind the segment
-        auto from = [&](long long cta) { return cta * kPagedWarps * total / workers; };
-        long long at = (end - 1) * ctas / total;
-        while (from(at + 1) <= end - 1)
-            ++at;
-        while (from(at) > end - 1)
-            --at;
-        descs[blockIdx.x] = PagedDesc{s_seg[warp][2], s_seg[warp][3], (int)(at - blockIdx.x) + 1, 0};
+        came_in = came_in && !s_works[w];
     }
-    if (!any_open && tid == 0)
+    if (!described && tid == 0)
         descs[blockIdx.x] = PagedDesc{0, 0, 0, 0};
 }
 
