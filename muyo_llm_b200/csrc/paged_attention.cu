@@ -40,6 +40,7 @@ struct PagedAttnDev {
     PagedDev c;
     int seqs, table_stride, window;
     int page_shift;  // log2(page_size), or -1
+    int one_page;    // whether every tile lies inside one page
     long long stride_q, stride_out;
     float scale;  // softmax scale * k_scale
 };
@@ -72,7 +73,6 @@ struct PagedTile {
     static_assert(KT % KSTEP == 0 && KT * CPR % 32 == 0, "tile shape");
     static_assert(RING >= PART * 4, "a drained ring holds a partial");
     static constexpr size_t SMEM = (size_t)kPagedWarps * (RING + PART * 4);
-    static_assert(SMEM >= kPagedThreads * 8, "the scan shares the rings");
 };
 
 template <int CPR>
@@ -188,18 +188,24 @@ struct PagedSpan {
     }
 };
 
+__device__ __forceinline__ float paged_lse(float m, float l)
+{
+    return l > 0.0f ? (m + log2f(l)) * 0.693147180559945f : -INFINITY;
+}
+
 // A tile of the batch: tile t of request s under KV head h.
 template <int KT>
 struct PagedCursor {
     int s, h, t;
     PagedSpan<KT> span;
-    // The next tile; the caller knows that there is one.
+    // Goes to the next tile, of which the caller knows; true at a segment's first.
     __device__ __forceinline__ bool next(const PagedAttnDev& p, const int32_t* lens)
     {
         if (++t < span.t1)
             return false;
         if (++h == p.c.kv_heads) {
             h = 0;
+#pragma unroll 1
             do {
                 span = PagedSpan<KT>(p, __ldg(lens + ++s));
             } while (span.t1 == span.t0);
@@ -209,59 +215,24 @@ struct PagedCursor {
     }
 };
 
-// Joins one row of the pieces of a segment, partials of the layout o [ROWS][HD], m [ROWS], l [ROWS]: a row's m is
-// the reference of its weights in log2 units, l their sum. piece(i) is asked for by lane i % 32 only.
-template <int HD, int ROWS, typename PieceAt, typename Emit>
-__device__ __forceinline__ void join_row(int r, int pieces, PieceAt piece, Emit emit)
-{
-    const int lane = threadIdx.x & 31;
-    float M = -INFINITY;
-    for (int i = lane; i < pieces; i += 32)
-        M = fmaxf(M, piece(i)[ROWS * HD + r]);
-    M = warp_max(M);
-    float L = 0.0f, o[(HD + 31) / 32];
-#pragma unroll
-    for (int e = 0; e < (HD + 31) / 32; ++e)
-        o[e] = 0.0f;
-    for (int i0 = 0; i0 < pieces; i0 += 32) {
-        float w = 0.0f, lw = 0.0f;  // lane i holds piece i0 + i's weight
-        const float* at = nullptr;
-        if (i0 + lane < pieces) {
-            at = piece(i0 + lane);
-            const float l = at[ROWS * HD + ROWS + r];
-            w = l > 0.0f ? ex2(at[ROWS * HD + r] - M) : 0.0f;
-            lw = l * w;
-        }
-        L += warp_sum(lw);
-        const int n = min(32, pieces - i0);
-#pragma unroll 8
-        for (int i = 0; i < n; ++i) {
-            const float wi = __shfl_sync(0xffffffffu, w, i);
-            const float* row =
-                reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(at), i)) + r * HD;
-#pragma unroll
-            for (int e = 0; e < (HD + 31) / 32; ++e)
-                if (HD % 32 == 0 || lane < HD)
-                    o[e] = fmaf(wi, row[lane + 32 * e], o[e]);
-        }
+// Contiguous shares of `total` tiles for `workers` warps: the first `extra` get one more.
+struct PagedShares {
+    unsigned each, extra;
+    __device__ __forceinline__ PagedShares(unsigned total, unsigned workers) : each(total / workers), extra(total % workers) {}
+    __device__ __forceinline__ int begin(unsigned worker) const { return (int)(worker * each + min(worker, extra)); }
+    __device__ __forceinline__ int worker_of(unsigned tile) const
+    {
+        const unsigned border = extra * (each + 1);
+        return (int)(tile < border ? tile / (each + 1) : extra + (tile - border) / each);
     }
-    emit(M, L, o);
-}
+};
 
-template <int HD>
-__device__ __forceinline__ void write_row(const PagedAttnDev& p, int s, int head, float M, float L,
-                                          const float (&o)[(HD + 31) / 32], float* out, float* lse)
-{
-    const int lane = threadIdx.x & 31;
-    const float inv = L > 0.0f ? __fdiv_rn(p.c.v_scale, L) : 0.0f;
-    float* dst = out + s * p.stride_out + (long long)head * HD;
-#pragma unroll
-    for (int e = 0; e < (HD + 31) / 32; ++e)
-        if (HD % 32 == 0 || lane < HD)
-            dst[lane + 32 * e] = o[e] * inv;
-    if (lse && lane == 0)
-        lse[(size_t)s * p.c.heads + head] = L > 0.0f ? (M + log2f(L)) * 0.693147180559945f : -INFINITY;
-}
+// Pieces of one segment that a CTA joins: bit w the first piece of warp w, bit 8 + w its last one.
+struct PagedGroup {
+    unsigned pieces;
+    int seq, kv_head;
+    int to;  // -1: complete; else the CTA's partial 0 (the segment came in) or 1 (it begins here)
+};
 
 template <int T, int HD, bool WIDE>
 __global__ void __launch_bounds__(kPagedThreads, 1)
@@ -271,141 +242,185 @@ k_paged_attention(PagedAttnDev p, const float* __restrict__ q, const char* __res
 {
     using C = PagedTile<T, HD, WIDE>;
     constexpr int KT = C::KT, HR = WIDE ? 2 : 1;  // HR: heads of a lane
+    constexpr int W = kPagedWarps;
     extern __shared__ __align__(128) char paged_smem[];
-    __shared__ unsigned long long s_mask[kPagedWarps][C::STAGES];
-    __shared__ int s_first[kPagedWarps], s_last[kPagedWarps];  // 0 none, 1 open at the end, 2 ends here
-    __shared__ int s_seg[kPagedWarps][4];                      // request and KV head of the first and the last piece
-    __shared__ int s_works[kPagedWarps];
-    __shared__ int s_open;                                     // tiles of the CTA's last segment behind its range
-    __shared__ long long s_warp[kPagedWarps];
+    __shared__ unsigned long long s_mask[W][C::STAGES];
+    __shared__ int s_sum[W], s_start[W][2];
+    __shared__ int s_first[W], s_last[W];  // open pieces: 0 none, 1 open at the end, 2 ends here
+    __shared__ int s_seg[W][4];            // request and KV head of the first and the last piece
+    __shared__ int s_open;                 // tiles of the CTA's last segment behind its range
+    __shared__ int s_groups;
+    __shared__ PagedGroup s_group[W + 1];
+    __shared__ float2 s_rows[(W + 1) * C::ROWS];
     pdl_wait();
     pdl_trigger();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, cq = lane & 3;
 
-    // The batch's tiles: scanned[i] of all requests up to the end of thread i's share.
-    long long* scanned = reinterpret_cast<long long*>(paged_smem);
+    // The batch's tiles, scanned over the threads' contiguous requests.
     const int per = (p.seqs + kPagedThreads - 1) / kPagedThreads;
-    long long mine = 0;
-    for (int s = tid * per; s < min(tid * per + per, p.seqs); ++s) {
+    const int s_begin = min(tid * per, p.seqs), s_end = min(s_begin + per, p.seqs);
+    int mine = 0, empty = 0;
+#pragma unroll 1
+    for (int s = s_begin; s < s_end; ++s) {
         const PagedSpan<KT> span(p, __ldg(lens + s));
-        mine += (long long)(span.t1 - span.t0) * p.c.kv_heads;
+        mine += (span.t1 - span.t0) * p.c.kv_heads;
+        empty |= span.t1 == span.t0;
     }
-    long long incl = mine;
+    int incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, incl, o);
+        const int y = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o)
             incl += y;
     }
     if (lane == 31)
-        s_warp[warp] = incl;
+        s_sum[warp] = incl;
+    if (tid < W)
+        s_first[tid] = s_last[tid] = 0;
     if (tid == 0)
         s_open = 0;
-    __syncthreads();
-    long long total = 0;
+    empty = __syncthreads_or(empty);
+    int total = 0;
 #pragma unroll
-    for (int w = 0; w < kPagedWarps; ++w) {
-        if (w < warp)
-            incl += s_warp[w];
-        total += s_warp[w];
+    for (int w = 0; w < W; ++w) {
+        const int v = s_sum[w];
+        incl += w < warp ? v : 0;
+        total += v;
     }
-    scanned[tid] = incl;
-    // Requests without keys.
-    for (int s = blockIdx.x * kPagedWarps + warp; s < p.seqs; s += gridDim.x * kPagedWarps) {
-        const PagedSpan<KT> span(p, __ldg(lens + s));
-        if (span.t1 > span.t0)
-            continue;
-        for (int d = lane; d < p.c.heads * HD; d += 32)
-            out[s * p.stride_out + d] = 0.0f;
-        if (lse)
-            for (int h = lane; h < p.c.heads; h += 32)
-                lse[(size_t)s * p.c.heads + h] = -INFINITY;
+    const int ctas = min((int)gridDim.x, (total + W - 1) / W);  // CTAs with work
+    const PagedShares shares((unsigned)total, (unsigned)max(ctas, 1) * W);
+    const int worker = blockIdx.x * W + warp;
+    const bool idle = (int)blockIdx.x >= ctas;
+    if (!idle && mine > 0) {  // the warps whose first tile is of this thread's requests
+        const int excl = incl - mine;
+#pragma unroll 1
+        for (int w = 0; w < W; ++w) {
+            int rest = shares.begin(blockIdx.x * W + w) - excl;
+            if (rest < 0 || rest >= mine)
+                continue;
+            int s = s_begin;
+#pragma unroll 1
+            for (;; ++s) {
+                const PagedSpan<KT> span(p, __ldg(lens + s));
+                const int tiles = (span.t1 - span.t0) * p.c.kv_heads;
+                if (rest < tiles)
+                    break;
+                rest -= tiles;
+            }
+            s_start[w][0] = s;
+            s_start[w][1] = rest;
+        }
     }
     __syncthreads();
-    const int ctas = (int)min((long long)gridDim.x, (total + kPagedWarps - 1) / kPagedWarps);  // CTAs with work
-    if ((int)blockIdx.x >= ctas) {
+    if (empty) {  // requests without keys
+#pragma unroll 1
+        for (int s = blockIdx.x * W + warp; s < p.seqs; s += gridDim.x * W) {
+            const PagedSpan<KT> span(p, __ldg(lens + s));
+            if (span.t1 > span.t0)
+                continue;
+#pragma unroll 1
+            for (int d = lane; d < p.c.heads * HD; d += 32)
+                out[s * p.stride_out + d] = 0.0f;
+            if (lse)
+#pragma unroll 1
+                for (int h = lane; h < p.c.heads; h += 32)
+                    lse[(size_t)s * p.c.heads + h] = -INFINITY;
+        }
+    }
+    if (idle) {
         if (tid == 0)
             descs[blockIdx.x] = PagedDesc{0, 0, 0, 0};
         return;
     }
-    const long long workers = (long long)ctas * kPagedWarps, worker = (long long)blockIdx.x * kPagedWarps + warp;
-    const long long u0 = worker * total / workers, u1 = (worker + 1) * total / workers;
-    const long long cta_end = ((long long)blockIdx.x + 1) * kPagedWarps * total / workers;
-    int left = (int)(u1 - u0), ahead = left;  // tiles to work on, to copy
+    const int cta_end = shares.begin((blockIdx.x + 1) * W);
+    const int u1 = shares.begin(worker + 1);
+    int left = u1 - shares.begin(worker), ahead = left;  // tiles to work on, to copy
     PagedCursor<KT> cur;
     if (left > 0) {
-        int lo = 0, hi = kPagedThreads - 1;  // the first share that reaches past u0
-        while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            if (scanned[mid] > u0)
-                hi = mid;
-            else
-                lo = mid + 1;
-        }
-        long long rest = u0 - (lo > 0 ? scanned[lo - 1] : 0);
-        cur.s = lo * per;
-        for (;;) {
-            cur.span = PagedSpan<KT>(p, __ldg(lens + cur.s));
-            const long long units = (long long)(cur.span.t1 - cur.span.t0) * p.c.kv_heads;
-            if (rest < units)
-                break;
-            rest -= units;
-            ++cur.s;
-        }
-        const int tiles = cur.span.t1 - cur.span.t0;
-        cur.h = (int)(rest / tiles);
-        cur.t = cur.span.t0 + (int)(rest % tiles);
+        cur.s = s_start[warp][0];
+        cur.span = PagedSpan<KT>(p, __ldg(lens + cur.s));
+        const int tiles = cur.span.t1 - cur.span.t0, rest = s_start[warp][1];
+        cur.h = rest / tiles;
+        cur.t = cur.span.t0 + rest - cur.h * tiles;
     }
-    __syncthreads();  // scanned is done with: the rings take its place
 
     char* ring = paged_smem + (size_t)warp * C::RING;
     const uint32_t ring_at = smem_addr(ring);
-    float* first_part = reinterpret_cast<float*>(paged_smem + (size_t)kPagedWarps * C::RING) + (size_t)warp * C::PART;
+    float* first_part = reinterpret_cast<float*>(paged_smem + (size_t)W * C::RING) + (size_t)warp * C::PART;
 
     // ---- copies ----
+    // A tile inside one page (page_size a multiple of KT) has its rows slot_stride apart from one place on; else each
+    // row's place comes from the lane that looked its page up.
+    constexpr int RPI = 32 / C::CPR;  // rows of one copy instruction
+    const int ch = lane % C::CPR, row0 = lane / C::CPR;
+    const long long slot_bytes = p.c.slot_stride * C::ES;
     PagedCursor<KT> load = cur;
     int pages[(KT + 31) / 32];
-    auto look_up = [&]() {
+    auto look_up = [&](bool begins) {
 #pragma unroll
         for (int i = 0; i < (KT + 31) / 32; ++i) {
-            const int key = load.t * KT + i * 32 + lane;
+            const int key = p.one_page ? load.t * KT : load.t * KT + i * 32 + lane;
+            const int at = p.page_shift >= 0 ? key >> p.page_shift : key / p.c.page_size;
             pages[i] = -1;
-            if ((KT % 32 == 0 || lane < KT) && key < load.span.n && key >= load.span.begin) {
-                const int at = p.page_shift >= 0 ? key >> p.page_shift : key / p.c.page_size;
+            if (p.one_page ? i == 0 : (KT % 32 == 0 || lane < KT) && key < load.span.n && key >= load.span.begin)
                 pages[i] = __ldg(table + (size_t)load.s * p.table_stride + at);
+        }
+        if (begins) {  // the segment's q into L1: behind the copies it would wait for them
+            const float* qrow = q + load.s * p.stride_q + (long long)load.h * p.c.group * HD;
+#pragma unroll 1
+            for (int d = lane * 32; d < p.c.group * HD; d += 32 * 32) {
+                float unused;
+                asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(unused) : "l"(qrow + d));
             }
         }
     };
     auto issue = [&](int stage) {
-        if (ahead > 0) {
+        const uint32_t kd = ring_at + stage * 2 * C::TILE, vd = kd + C::TILE;
+        unsigned long long mask = 0;
+        const int key0 = load.t * KT;
+        if (p.one_page) {
+            const bool ok = pages[0] >= 0 && pages[0] < p.c.num_pages;
+            const int slot = p.page_shift >= 0 ? key0 & (p.c.page_size - 1) : key0 % p.c.page_size;
+            const int lo = ok ? load.span.begin - key0 : KT, hi = load.span.n - key0;  // rows lo .. hi - 1 are seen
+            long long o = ok ? (pages[0] * p.c.page_stride + load.h * p.c.head_stride + (slot + row0) * p.c.slot_stride) * C::ES
+                             : 0;
+            o += ch * 16;
+#pragma unroll
+            for (int i = 0; i < (KT + 31) / 32; ++i)
+                mask |= (unsigned long long)__ballot_sync(0xffffffffu, i * 32 + lane >= lo && i * 32 + lane < min(hi, KT))
+                        << (32 * i);
+#pragma unroll
+            for (int i = 0; i < KT * C::CPR / 32; ++i) {
+                const int row = i * RPI + row0;
+                const bool seen = row >= lo && row < hi;
+                copy16(kd + row * C::RB + k_chunk<C::CPR>(row, ch) * 16, k_pool + (seen ? o : 0), seen);
+                copy16(vd + row * C::RB + v_chunk<C::CPR>(row, ch) * 16, v_pool + (seen ? o : 0), seen);
+                o += RPI * slot_bytes;
+            }
+        } else {
             long long off[(KT + 31) / 32];
-            unsigned long long mask = 0;
 #pragma unroll
             for (int i = 0; i < (KT + 31) / 32; ++i) {
-                const int key = load.t * KT + i * 32 + lane;
+                const int key = key0 + i * 32 + lane;
                 const int slot = p.page_shift >= 0 ? key & (p.c.page_size - 1) : key % p.c.page_size;
                 const bool ok = pages[i] >= 0 && pages[i] < p.c.num_pages;
                 off[i] = ok ? (pages[i] * p.c.page_stride + load.h * p.c.head_stride + slot * p.c.slot_stride) * C::ES : 0;
                 mask |= (unsigned long long)__ballot_sync(0xffffffffu, ok) << (32 * i);
             }
-            if (lane == 0)
-                s_mask[warp][stage] = mask;
-            const uint32_t kd = ring_at + stage * 2 * C::TILE, vd = kd + C::TILE;
 #pragma unroll
             for (int i = 0; i < KT * C::CPR / 32; ++i) {
-                const int row = (i * 32 + lane) / C::CPR, ch = (i * 32 + lane) % C::CPR;
-                const long long o = __shfl_sync(0xffffffffu, off[i * 32 / C::CPR / 32], row & 31) + ch * 16;
-                const bool ok = (mask >> row) & 1;
-                copy16(kd + row * C::RB + k_chunk<C::CPR>(row, ch) * 16, k_pool + (ok ? o : 0), ok);
-                copy16(vd + row * C::RB + v_chunk<C::CPR>(row, ch) * 16, v_pool + (ok ? o : 0), ok);
-            }
-            if (--ahead > 0) {
-                load.next(p, lens);
-                look_up();
+                const int row = i * RPI + row0;
+                const long long o = __shfl_sync(0xffffffffu, off[i * RPI / 32], row & 31) + ch * 16;
+                const bool seen = (mask >> row) & 1;
+                copy16(kd + row * C::RB + k_chunk<C::CPR>(row, ch) * 16, k_pool + (seen ? o : 0), seen);
+                copy16(vd + row * C::RB + v_chunk<C::CPR>(row, ch) * 16, v_pool + (seen ? o : 0), seen);
             }
         }
-        copies_commit();
+        if (lane == 0)
+            s_mask[warp][stage] = mask;
+        if (--ahead > 0)
+            look_up(load.next(p, lens));
     };
 
     // ---- the segment at hand ----
@@ -691,58 +706,56 @@ k_paged_attention(PagedAttnDev p, const float* __restrict__ q, const char* __res
 
     // Writes the segment's result: to `out` when it is complete, else as a partial.
     auto end_segment = [&](float* partial) {
+        float* dst = partial ? partial : out + cur.s * p.stride_out + (long long)cur.h * p.c.group * HD;
 #pragma unroll
         for (int r = 0; r < HR; ++r) {
             const int head = g + 8 * r;
-            float L = l[r];
+            float L = l[r], by = 1.0f;
             L += __shfl_xor_sync(0xffffffffu, L, 1);
             L += __shfl_xor_sync(0xffffffffu, L, 2);
-            float* dst;
-            float by = 1.0f;
-            if (partial) {
-                dst = partial + head * HD;
-                if (cq == 0) {
-                    partial[C::ROWS * HD + head] = m[r];
-                    partial[C::ROWS * HD + C::ROWS + head] = L;
-                }
-            } else {
-                if (head >= p.c.group)
-                    continue;
-                const int h = cur.h * p.c.group + head;
-                dst = out + cur.s * p.stride_out + (long long)h * HD;
-                by = L > 0.0f ? __fdiv_rn(p.c.v_scale, L) : 0.0f;
-                if (lse && cq == 0)
-                    lse[(size_t)cur.s * p.c.heads + h] = L > 0.0f ? (m[r] + log2f(L)) * 0.693147180559945f : -INFINITY;
-            }
-#pragma unroll
-            for (int ic = 0; ic < C::NVC; ++ic)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int d = (8 * ic + 2 * cq + e) * C::VE;
-                    if constexpr (C::VE >= 4) {
-#pragma unroll
-                        for (int n = 0; n < C::VE; n += 4)
-                            *reinterpret_cast<float4*>(dst + d + n) =
-                                make_float4(o[ic * C::VE + n][2 * r + e] * by, o[ic * C::VE + n + 1][2 * r + e] * by,
-                                            o[ic * C::VE + n + 2][2 * r + e] * by, o[ic * C::VE + n + 3][2 * r + e] * by);
-                    } else {
-#pragma unroll
-                        for (int n = 0; n < C::VE; ++n)
-                            dst[d + n] = o[ic * C::VE + n][2 * r + e] * by;
+            if (head < p.c.group) {
+                if (partial) {
+                    if (cq == 0) {
+                        partial[C::ROWS * HD + head] = m[r];
+                        partial[C::ROWS * HD + C::ROWS + head] = L;
                     }
+                } else {
+                    by = L > 0.0f ? __fdiv_rn(p.c.v_scale, L) : 0.0f;
+                    if (lse && cq == 0)
+                        lse[(size_t)cur.s * p.c.heads + cur.h * p.c.group + head] = paged_lse(m[r], L);
                 }
+#pragma unroll
+                for (int ic = 0; ic < C::NVC; ++ic)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float* at = dst + head * HD + (8 * ic + 2 * cq + e) * C::VE;
+                        if constexpr (C::VE >= 4) {
+#pragma unroll
+                            for (int n = 0; n < C::VE; n += 4)
+                                *reinterpret_cast<float4*>(at + n) =
+                                    make_float4(o[ic * C::VE + n][2 * r + e] * by, o[ic * C::VE + n + 1][2 * r + e] * by,
+                                                o[ic * C::VE + n + 2][2 * r + e] * by, o[ic * C::VE + n + 3][2 * r + e] * by);
+                        } else {
+#pragma unroll
+                            for (int n = 0; n < C::VE; ++n)
+                                at[n] = o[ic * C::VE + n][2 * r + e] * by;
+                        }
+                    }
+            }
         }
     };
 
-    int first = 0, last = 0;  // this warp's open pieces
     if (left > 0) {
-        look_up();
-#pragma unroll
-        for (int i = 0; i < C::STAGES - 1; ++i)
-            issue(i);
-        int stage = 0, into = C::STAGES - 1;
-        while (left > 0) {
-            issue(into);
+        look_up(true);
+        int stage = 0, into = 0;
+#pragma unroll 1
+        for (int step = 1 - C::STAGES; left > 0; ++step) {
+            if (ahead > 0)
+                issue(into);
+            copies_commit();
+            into = into + 1 == C::STAGES ? 0 : into + 1;
+            if (step < 0)
+                continue;
             if (fresh)
                 begin_segment();
             copies_wait<C::STAGES - 1>();
@@ -750,123 +763,184 @@ k_paged_attention(PagedAttnDev p, const float* __restrict__ q, const char* __res
             tile(stage);
             __syncwarp();  // every lane is done with the stage before it is filled again
             stage = stage + 1 == C::STAGES ? 0 : stage + 1;
-            into = into + 1 == C::STAGES ? 0 : into + 1;
             --left;
             const bool ends = cur.t + 1 == cur.span.t1;
             fresh = ends;
             if (ends || left == 0) {
-                if (whole && ends) {
-                    end_segment(nullptr);
-                } else if (!whole) {
-                    first = ends ? 2 : 1;
-                    if (lane == 0)
-                        s_seg[warp][0] = cur.s, s_seg[warp][1] = cur.h;
-                    end_segment(first_part);
-                } else {  // begun here, open: the ring is drained
-                    last = 1;
-                    if (lane == 0)
-                        s_seg[warp][2] = cur.s, s_seg[warp][3] = cur.h;
-                    end_segment(reinterpret_cast<float*>(ring));
+                if (!(whole && ends) && lane == 0) {
+                    const int k = whole ? 2 : 0;
+                    s_seg[warp][k] = cur.s, s_seg[warp][k + 1] = cur.h;
+                    (whole ? s_last : s_first)[warp] = ends ? 2 : 1;
+                    if (!ends && u1 == cta_end)
+                        s_open = cur.span.t1 - cur.t - 1;
                 }
+                // a piece that begins here and is open goes to the ring, which is drained then
+                end_segment(whole && ends ? nullptr : whole ? reinterpret_cast<float*>(ring) : first_part);
             }
             if (left > 0)
                 cur.next(p, lens);
-            else if (!ends && u1 == cta_end && lane == 0)
-                s_open = cur.span.t1 - cur.t - 1;
         }
-    }
-    if (lane == 0) {
-        s_first[warp] = first;
-        s_last[warp] = last;
-        s_works[warp] = u1 > u0;
     }
     __syncthreads();
 
     // ---- the CTA's join ----
-    // A group is a piece that begins here (or, in the first warp with work, comes in) and the first pieces of the warps
-    // behind it, up to the one where the segment ends. Every warp takes rows of every group.
-    bool came_in = true;  // no warp before w had work
-    bool described = false;
-    int turn = 0;
-    for (int w = 0; w < kPagedWarps; ++w) {
-        for (int kind = 0; kind < 2; ++kind) {
-            const bool incoming = kind == 0;
-            if (incoming ? !(came_in && s_first[w]) : !s_last[w])
+    // A group is a piece that begins here (or comes in, to warp 0) and the first pieces of the warps behind it, up to the
+    // one where the segment ends.
+    if (tid == 0) {
+        int groups = 0;
+        PagedDesc desc{0, 0, 0, 0};
+#pragma unroll 1
+        for (int k = -1; k < W; ++k) {  // -1: what comes in
+            const int w = max(k, 0);
+            if (k < 0 ? !s_first[0] : !s_last[w])
                 continue;
-            bool ended = incoming && s_first[w] == 2;
-            int pieces = 1, from = w;  // from: the warp of this lane's piece
-            for (int v = w + 1; v < kPagedWarps && !ended; ++v) {
-                if (s_first[v]) {
-                    from = pieces == lane ? v : from;
-                    ++pieces;
-                    ended = s_first[v] == 2;
-                }
+            bool ended = k < 0 && s_first[0] == 2;
+            unsigned pieces = 1u << (k < 0 ? 0 : 8 + w);
+#pragma unroll 1
+            for (int v = w + 1; v < W && !ended; ++v) {
+                pieces |= s_first[v] ? 1u << v : 0u;
+                ended = s_first[v] == 2;
             }
-            const int seq = s_seg[w][incoming ? 0 : 2], kvh = s_seg[w][incoming ? 1 : 3];
-            auto piece = [&](int i) -> const float* {
-                return reinterpret_cast<const float*>(
-                    incoming || i > 0 ? paged_smem + (size_t)kPagedWarps * C::RING + (size_t)from * C::PART * 4
-                                      : paged_smem + (size_t)from * C::RING);
-            };
-            float* to = part + ((size_t)blockIdx.x * 2 + (incoming ? 0 : 1)) * C::PART;
-            const bool complete = ended && !incoming;
-            for (int r = 0; r < p.c.group; ++r) {
-                if ((turn++ & (kPagedWarps - 1)) != warp)
-                    continue;
-                join_row<HD, C::ROWS>(r, pieces, piece, [&](float M, float L, const float(&v)[(HD + 31) / 32]) {
-                    if (complete) {
-                        write_row<HD>(p, seq, kvh * p.c.group + r, M, L, v, out, lse);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < (HD + 31) / 32; ++e)
-                            if (HD % 32 == 0 || lane < HD)
-                                to[r * HD + lane + 32 * e] = v[e];
-                        if (lane == 0) {
-                            to[C::ROWS * HD + r] = M;
-                            to[C::ROWS * HD + C::ROWS + r] = L;
-                        }
-                    }
-                });
-            }
-            if (!ended && !incoming) {  // begun in this CTA and open behind it (one group at most): who joins it
-                described = true;
-                if (tid == 0) {
-                    const long long end = cta_end + s_open;  // behind the segment
-                    auto begin = [&](long long cta) { return cta * kPagedWarps * total / workers; };
-                    long long at = (end - 1) * ctas / total;
-                    while (begin(at + 1) <= end - 1)
-                        ++at;
-                    while (begin(at) > end - 1)
-                        --at;
-                    descs[blockIdx.x] = PagedDesc{seq, kvh, (int)(at - blockIdx.x) + 1, 0};
-                }
+            const PagedGroup group{pieces, s_seg[w][k < 0 ? 0 : 2], s_seg[w][k < 0 ? 1 : 3], k < 0 ? 0 : ended ? -1 : 1};
+            s_group[groups++] = group;
+            if (group.to == 1) {  // begun in this CTA and open behind it: one group at most
+                const int to = shares.worker_of((unsigned)(cta_end + s_open - 1)) / W;
+                desc = PagedDesc{group.seq, group.kv_head, to - (int)blockIdx.x + 1, 0};
             }
         }
-        came_in = came_in && !s_works[w];
+        s_groups = groups;
+        descs[blockIdx.x] = desc;
     }
-    if (!described && tid == 0)
-        descs[blockIdx.x] = PagedDesc{0, 0, 0, 0};
+    __syncthreads();
+    const int rows = s_groups * p.c.group;
+    // The pieces' weights 2^(m - M), in place of m, by 16 lanes per row; M and L by the group's first piece.
+    auto piece_at = [&](int b) -> float* {
+        return reinterpret_cast<float*>(b < 8 ? paged_smem + (size_t)W * C::RING + (size_t)b * C::PART * 4
+                                              : paged_smem + (size_t)(b - 8) * C::RING);
+    };
+    static_assert(W == 8, "a piece per lane of 16");
+    float* s_row = reinterpret_cast<float*>(s_rows);
+#pragma unroll 1
+    for (int i = tid >> 4; i < ((rows + 1) & ~1); i += kPagedThreads / 16) {
+        const int k = min(i, rows - 1) / p.c.group, r = min(i, rows - 1) % p.c.group, b = lane & 15;
+        const bool in = (s_group[k].pieces >> b) & 1;
+        float* at = piece_at(b) + C::ROWS * HD + r;
+        float m1 = in ? at[0] : -INFINITY, l1 = in ? at[C::ROWS] : 0.0f, M = m1;
+#pragma unroll
+        for (int o2 = 8; o2 > 0; o2 >>= 1)
+            M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o2));
+        const float w = l1 > 0.0f ? ex2(m1 - M) : 0.0f;
+        float L = l1 * w;
+#pragma unroll
+        for (int o2 = 8; o2 > 0; o2 >>= 1)
+            L += __shfl_xor_sync(0xffffffffu, L, o2);
+        if (i < rows) {
+            if (in)
+                at[0] = w;
+            if (b == 0) {
+                s_row[2 * i] = M;
+                s_row[2 * i + 1] = L;
+            }
+        }
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int i = tid; i < rows * (HD / 4); i += kPagedThreads) {
+        const int row = i / (HD / 4), d = i % (HD / 4) * 4;
+        const int k = row / p.c.group, r = row % p.c.group;
+        const PagedGroup group = s_group[k];
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+        for (unsigned bits = group.pieces; bits; bits &= bits - 1) {
+            const float* at = piece_at(__ffs(bits) - 1);
+            const float w = at[C::ROWS * HD + r];
+            const float4 x = *reinterpret_cast<const float4*>(at + r * HD + d);
+            v.x = fmaf(w, x.x, v.x), v.y = fmaf(w, x.y, v.y), v.z = fmaf(w, x.z, v.z), v.w = fmaf(w, x.w, v.w);
+        }
+        const float M = s_row[2 * row], L = s_row[2 * row + 1];
+        float* dst = part + ((size_t)blockIdx.x * 2 + group.to) * C::PART + r * HD;
+        if (group.to < 0) {
+            const int h = group.kv_head * p.c.group + r;
+            const float by = L > 0.0f ? __fdiv_rn(p.c.v_scale, L) : 0.0f;
+            v.x *= by, v.y *= by, v.z *= by, v.w *= by;
+            dst = out + group.seq * p.stride_out + (long long)h * HD;
+            if (lse && d == 0)
+                lse[(size_t)group.seq * p.c.heads + h] = paged_lse(M, L);
+        } else if (d == 0) {
+            dst[C::ROWS * HD - r * HD + r] = M;
+            dst[C::ROWS * HD - r * HD + C::ROWS + r] = L;
+        }
+        *reinterpret_cast<float4*>(dst + d) = v;
+    }
 }
 
 // Joins the segment that begins in CTA blockIdx.x of the kernel above and ends in another: its last partial and the
-// first ones of the CTAs behind it. A warp per query head.
+// first ones of the CTAs behind it. Four channels of a row per thread; threads to spare share the pieces.
+constexpr int kJoinThreads = 512;
+constexpr int kJoinPieces = 256;  // one per CTA at most
+
 template <int HD, int ROWS>
-__global__ void __launch_bounds__(ROWS * 32) k_paged_join(PagedAttnDev p, const float* __restrict__ part,
-                                                          const PagedDesc* __restrict__ descs, float* __restrict__ out,
-                                                          float* __restrict__ lse)
+__global__ void __launch_bounds__(kJoinThreads) k_paged_join(PagedAttnDev p, const float* __restrict__ part,
+                                                             const PagedDesc* __restrict__ descs, float* __restrict__ out,
+                                                             float* __restrict__ lse)
 {
-    constexpr int PART = ROWS * (HD + 2);
+    constexpr int PART = ROWS * (HD + 2), Q = HD / 4;
+    __shared__ float s_w[ROWS][kJoinPieces];
+    __shared__ float s_L[ROWS];
+    __shared__ float4 s_sum[kJoinThreads];
     pdl_wait();
     pdl_trigger();
     const PagedDesc d = descs[blockIdx.x];
-    const int r = threadIdx.x >> 5;
-    if (d.pieces == 0 || r >= p.c.group)
+    if (d.pieces == 0)
         return;
-    const size_t at = blockIdx.x;
-    auto piece = [&](int i) -> const float* { return part + (i == 0 ? at * 2 + 1 : (at + i) * 2) * PART; };
-    join_row<HD, ROWS>(r, d.pieces, piece, [&](float M, float L, const float(&v)[(HD + 31) / 32]) {
-        write_row<HD>(p, d.seq, d.kv_head * p.c.group + r, M, L, v, out, lse);
-    });
+    const int tid = threadIdx.x, lane = tid & 31, G = p.c.group;
+    auto piece = [&](int i) { return part + ((size_t)blockIdx.x + i) * 2 * PART + (i == 0 ? PART : 0); };
+    const int items = G * Q, ways = items >= kJoinThreads ? 1 : kJoinThreads / items;
+    const int way = tid / items, item = tid % items;
+    if (tid >> 5 < G) {  // a warp per row: the pieces' weights
+        const int r = tid >> 5;
+        float M = -INFINITY, L = 0.0f;
+#pragma unroll 1
+        for (int i = lane; i < d.pieces; i += 32)
+            M = fmaxf(M, piece(i)[ROWS * HD + r]);
+        M = warp_max(M);
+#pragma unroll 1
+        for (int i = lane; i < d.pieces; i += 32) {
+            const float* at = piece(i) + ROWS * HD + r;
+            const float l = at[ROWS], w = l > 0.0f ? ex2(at[0] - M) : 0.0f;
+            s_w[r][i] = w;
+            L = fmaf(l, w, L);
+        }
+        L = warp_sum(L);
+        if (lane == 0) {
+            s_L[r] = L;
+            if (lse)
+                lse[(size_t)d.seq * p.c.heads + d.kv_head * G + r] = paged_lse(M, L);
+        }
+    }
+    __syncthreads();
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (way < ways) {
+#pragma unroll 8
+        for (int i = way; i < d.pieces; i += ways) {
+            const float w = s_w[item / Q][i];
+            const float4 x = *reinterpret_cast<const float4*>(piece(i) + item * 4);
+            v.x = fmaf(w, x.x, v.x), v.y = fmaf(w, x.y, v.y), v.z = fmaf(w, x.z, v.z), v.w = fmaf(w, x.w, v.w);
+        }
+    }
+    s_sum[tid] = v;
+    __syncthreads();
+    if (tid < items) {
+#pragma unroll 1
+        for (int i = 1; i < ways; ++i) {
+            const float4 x = s_sum[i * items + tid];
+            v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+        }
+        const int r = item / Q;
+        const float by = s_L[r] > 0.0f ? __fdiv_rn(p.c.v_scale, s_L[r]) : 0.0f;
+        *reinterpret_cast<float4*>(out + d.seq * p.stride_out + (long long)(d.kv_head * G + r) * HD + item % Q * 4) =
+            make_float4(v.x * by, v.y * by, v.z * by, v.w * by);
+    }
 }
 
 static int paged_attention_prepare(const MuyoPagedAttentionParams* p, PagedAttnDev& d)
@@ -885,6 +959,12 @@ static int paged_attention_prepare(const MuyoPagedAttentionParams* p, PagedAttnD
     d.stride_out = p->stride_out ? p->stride_out : row;
     MUYO_REQUIRE(d.stride_q >= row && d.stride_out >= row, "paged_attention: a row stride is below the row of %u", row);
     MUYO_REQUIRE((d.stride_q | d.stride_out) % 4 == 0, "paged_attention: row strides must be multiples of 4");
+    // tiles hold 8 keys or more
+    const uint64_t tiles = ((uint64_t)p->cache.page_size * p->table_stride / 8 + 1) * p->cache.kv_heads;
+    if (tiles > (uint64_t)INT_MAX / p->seqs) {
+        set_error("paged_attention: %u requests of rows of %u pages are more than 2^31 tiles", p->seqs, p->table_stride);
+        return MUYO_EUNSUPPORTED;
+    }
     d.seqs = (int)p->seqs, d.table_stride = (int)p->table_stride, d.window = (int)p->window;
     d.scale = p->scale * d.c.k_scale;
     d.page_shift = -1;
@@ -897,9 +977,10 @@ static int paged_attention_prepare(const MuyoPagedAttentionParams* p, PagedAttnD
 // CTAs: one per SM, fewer when the tables could not hold a tile per warp.
 static int paged_attention_ctas(const PagedAttnDev& d)
 {
-    const long long tiles = ((long long)d.table_stride * d.c.page_size + 7) / 8 * d.c.kv_heads;
+    const long long tiles = ((long long)d.table_stride * d.c.page_size / 8 + 1) * d.c.kv_heads;
     const long long most = (tiles * d.seqs + kPagedWarps - 1) / kPagedWarps;
-    return (int)(most < sm_count() ? most : sm_count());
+    const int sms = sm_count() < kJoinPieces ? sm_count() : kJoinPieces;
+    return (int)(most < sms ? most : sms);
 }
 
 static size_t paged_attention_parts(const PagedAttnDev& d)
@@ -915,12 +996,14 @@ static int launch_paged_attention(const PagedAttnDev& d, const float* q, const v
     auto kernel = k_paged_attention<T, HD, WIDE>;
     MUYO_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM));
     const int ctas = paged_attention_ctas(d);
+    PagedAttnDev e = d;
+    e.one_page = d.c.page_size % C::KT == 0;
     float* part = static_cast<float*>(ws);
     PagedDesc* descs = reinterpret_cast<PagedDesc*>(static_cast<char*>(ws) + paged_attention_parts(d));
-    MUYO_CUDA_TRY(launch_kernel(kernel, dim3(ctas), dim3(kPagedThreads), C::SMEM, as_stream(stream), true, d, q,
+    MUYO_CUDA_TRY(launch_kernel(kernel, dim3(ctas), dim3(kPagedThreads), C::SMEM, as_stream(stream), true, e, q,
                                 static_cast<const char*>(k), static_cast<const char*>(v), table, lens, out, lse, part, descs));
     MUYO_LAUNCH_CHECK();
-    MUYO_CUDA_TRY(launch_kernel(k_paged_join<HD, C::ROWS>, dim3(ctas), dim3(C::ROWS * 32), 0, as_stream(stream), true, d,
+    MUYO_CUDA_TRY(launch_kernel(k_paged_join<HD, C::ROWS>, dim3(ctas), dim3(kJoinThreads), 0, as_stream(stream), true, d,
                                 part, descs, out, lse));
     MUYO_LAUNCH_CHECK();
     return MUYO_OK;
