@@ -571,7 +571,7 @@ typedef struct MuyoTokenLogprobsParams {
     uint32_t rows, vocab;
     uint32_t stride; /* 0 = vocab */
     uint32_t top_k;
-    float temperature; /* > 0 */
+    float temperature; /* 1e-6 .. 1e6 */
 } MuyoTokenLogprobsParams;
 size_t muyo_cuda_token_logprobs_workspace_size(const MuyoTokenLogprobsParams* p);
 int muyo_cuda_token_logprobs(const MuyoTokenLogprobsParams* p, const float* logits, const int32_t* tokens, float* logprob,
