@@ -1,8 +1,14 @@
 // Log probabilities of given tokens with entropy, rank and the top alternatives.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+#include <cfloat>
 #include <climits>
 #include <cmath>
 
 #include "common.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace muyo {
 
@@ -10,9 +16,10 @@ constexpr int kLogprobThreads = 256;
 constexpr int kLogprobWarps = kLogprobThreads / 32;
 constexpr int kLogprobJoinThreads = 128;
 constexpr int kLogprobMaxTop = 32;
-constexpr int kLogprobGroups = 64;   // groups of 4 threads whose maxima give the first threshold
-constexpr int kLogprobKeep = 256;    // keys that the list may carry from tile to tile: a thread each
-constexpr int kLogprobMaxTiles = 64; // of a piece
+constexpr int kLogprobGroups = 64;  // groups of 4 threads whose maxima give the threshold
+constexpr int kLogprobList = 512;   // listed logits
+constexpr int kLogprobMaxTiles = 64;  // of a piece
+constexpr int kLogprobCluster = 8;
 
 struct LogprobDev {
     int rows, vocab, top_k;
@@ -20,7 +27,8 @@ struct LogprobDev {
     float inv_t;  // log2(e) / temperature
     float temperature;
     int pieces, tiles;  // of a row; of a piece
-    bool small;         // tiles of 2048 logits instead of 4096
+    bool small;         // tiles of two float4 per thread instead of four
+    bool cluster;       // a row's pieces are one thread-block cluster, which joins them itself
 };
 
 struct LogprobOut {
@@ -72,6 +80,27 @@ __device__ __forceinline__ float weight_up(float u, float inv_t)
 }
 constexpr float kLogprobLeast = -1.0e29f;  // u where the weight is 0, so that 0 * -inf does not arise
 
+// The ids below `end` from `begin` on at which x is `value`, in order, by one warp: lanes have .. top_k - 1 receive them
+// (-1 without one).
+__device__ __forceinline__ int logprob_equal_ids(const float* x, float value, int begin, int end, int have, int top_k)
+{
+    const int lane = threadIdx.x & 31;
+    int id = -1;
+#pragma unroll 1
+    for (int i = begin; have < top_k && i < end; i += 32) {
+        const unsigned equal = __ballot_sync(0xffffffffu, i + lane < end && __ldg(x + min(i + lane, end - 1)) == value);
+        if (lane >= have && lane < top_k && lane - have < __popc(equal)) {
+            unsigned bits = equal;
+#pragma unroll 1
+            for (int k = have; k < lane; ++k)
+                bits &= bits - 1;
+            id = i + __ffs(bits) - 1;
+        }
+        have = min(have + __popc(equal), top_k);
+    }
+    return id;
+}
+
 // A row's results from its sums. log p = (x - m) / T - log(1 + r), where nothing is lost of r when it is far
 // below 1; H = log(1 + r) - e / (T (1 + r)).
 struct LogprobRow {
@@ -96,99 +125,337 @@ struct LogprobRow {
         if (out.rank)
             out.rank[row] = inside ? q.before : p.vocab;
     }
-    __device__ __forceinline__ void write_top(const LogprobOut& out, size_t at, unsigned long long key) const
+    // The first top_k ids by one warp, lane k the k-th; key 0 where no logit above -inf is left. Those places go to the
+    // lowest ids at -inf, read from the row x; -1 where there are none (NaN).
+    __device__ __forceinline__ void write_top(const LogprobDev& p, const LogprobOut& out, int row, unsigned long long key,
+                                              const float* x) const
     {
-        out.top_ids[at] = key ? (int)~(unsigned)key : -1;
-        out.top_logprobs[at] = log_p(key ? key_logit(key) : NAN);
+        const int lane = threadIdx.x & 31;
+        const int have = __popc(__ballot_sync(0xffffffffu, key != 0ull && lane < p.top_k));
+        int id = key ? (int)~(unsigned)key : -1;
+        float v = key ? key_logit(key) : NAN;
+        const int masked = logprob_equal_ids(x, -INFINITY, 0, p.vocab, have, p.top_k);
+        if (masked >= 0) {
+            id = masked;
+            v = -INFINITY;
+        }
+        if (lane < p.top_k) {
+            out.top_ids[(size_t)row * p.top_k + lane] = id;
+            out.top_logprobs[(size_t)row * p.top_k + lane] = log_p(v);
+        }
     }
 };
 
-// One piece of a row, read once: `tiles` tiles of V float4 per thread, the next one's loads under way while one is
-// worked on. A thread keeps its largest logit so far and its sums of w and w (x - m) relative to it. An id
-// below the token is in front of it at an equal logit too: it is compared with the next value below the token's.
+// Joins the sums of up to 32 pieces, by one warp: lane i has piece i's.
+__device__ __forceinline__ LogprobPiece logprob_join_sums(const LogprobDev& p, LogprobPiece q, int pieces)
+{
+    const bool here = (int)(threadIdx.x & 31) < pieces;
+    if (!here)
+        q = LogprobPiece{-INFINITY, 0.0f, 0.0f, 0};
+    const float m = warp_max(q.m), ms = m == -INFINITY ? 0.0f : m;
+    const bool top = here && q.m == m;
+    const float u = fmaxf(q.m - ms, kLogprobLeast), w = here ? weight_up(u, p.inv_t) : 0.0f;
+    LogprobPiece sum{m, 0.0f, 0.0f, 0};
+    sum.r = warp_sum(top ? q.r : (1.0f + q.r) * w * kLogprobDown) + (float)(__popc(__ballot_sync(0xffffffffu, top)) - 1);
+    sum.e = warp_sum(top ? q.e : fmaf(u, 1.0f + q.r, q.e) * w * kLogprobDown);
+    sum.before = __reduce_add_sync(0xffffffffu, q.before);
+    return sum;
+}
+
+// One piece of a row: tiles of V float4 per thread, two tiles' loads under way, no barrier. A thread keeps its largest
+// logit so far, its sums of w and w (x - m) relative to it, and its count of ids in front of the token (looked
+// at where a tile's largest is not below the token's logit). Where little lies beside the largest, its 1 has
+// rounded the sum: then the sums are formed again without it, from a second read.
 //
-// The first top_k ids: in the first tile the maxima of 64 groups of 4 threads give a threshold, the
-// top_k-th largest of them, that top_k logits reach and few others do (24 on average for 20 of 64 groups);
-// later tiles list what lies above it (an equal logit of a later id comes behind). A list past
-// kLogprobKeep keys is cut to its first top_k, whose last is the new threshold. A first tile with masses
-// at the threshold (a mask's -inf, a constant row) lists the logits above it, and of the equal ones the lowest ids.
-//
-// Bound by the read: 4 bytes a logit, 13 instructions.
-template <int V>
+// The first top_k ids: the threads' maxima, taken over 64 groups of 4 threads, give a threshold, the top_k-th
+// largest of them, that top_k logits reach and few others do (24 on average for 20 of 64). A warp
+// reads the logits of one such thread at a time again, a float4 per lane; those that reach the threshold
+// are ordered by counting. -inf is never listed, its places are filled in at the end. Masses at the threshold (a
+// constant row, a mask of the lowest value) run the list over: then what lies above it is listed, and of the equal
+// ones the lowest ids.
+template <bool TOP, int V>
 __global__ void __launch_bounds__(kLogprobThreads, 4) k_logprob_pieces(LogprobDev p, const float* __restrict__ logits,
                                                                        const int32_t* __restrict__ tokens,
                                                                        LogprobPiece* __restrict__ stats,
                                                                        unsigned long long* __restrict__ tops, LogprobOut out)
 {
-    constexpr int WARPS = kLogprobWarps, TILE = kLogprobThreads * 4 * V;
-    __shared__ float s_m[WARPS], s_r[WARPS], s_e[WARPS], s_group[kLogprobGroups], s_threshold;
-    __shared__ int s_before[WARPS], s_equal[WARPS], s_count, s_above, s_ties[WARPS];
-    __shared__ unsigned long long s_key[WARPS], s_top[kLogprobMaxTop];
-    extern __shared__ unsigned long long s_list[];  // [kLogprobKeep + TILE] when top_k > 0
+    constexpr int WARPS = kLogprobWarps, Q = kLogprobThreads * 4, TILE = V * Q;
+    __shared__ float s_m[WARPS], s_r[WARPS], s_e[WARPS], s_mine[TOP ? kLogprobThreads : 1], s_threshold;
+    __shared__ int s_before[WARPS], s_count, s_threads, s_thread[TOP ? kLogprobThreads : 1];
+    __shared__ unsigned long long s_key[WARPS], s_top[kLogprobMaxTop], s_list[TOP ? kLogprobList : 1];
+    __shared__ LogprobPiece s_sum;
     pdl_wait();
     pdl_trigger();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int row = blockIdx.x / p.pieces, piece = blockIdx.x - row * p.pieces;
     const float* x = logits + row * p.stride;
-    const int token = __ldg(tokens + row);  // not waited for before the first tile's loads are under way
-    // float4 from the 16-byte border at or before the row's first logit
-    const int shift = (int)((reinterpret_cast<uintptr_t>(x) >> 2) & 3);
-    const int first = piece * p.tiles * TILE - shift, end = min(first + p.tiles * TILE, p.vocab);
-    int base = first + tid * 4;  // of the tile at hand: id of bit 0
-    const auto load = [&](float (&v)[V][4], int at) {
-        const int tile = at - tid * 4;
-        if (tile >= 0 && tile + TILE <= p.vocab) {
+    const int token = __ldg(tokens + row);
+    // float4 from the 16-byte border at or before the row's first logit; ids outside [begin, end) read as -inf
+    const int origin = piece * p.tiles * TILE - (int)((reinterpret_cast<uintptr_t>(x) >> 2) & 3);
+    const int begin = max(origin, 0), end = min(origin + p.tiles * TILE, p.vocab);
+    const int tiles = (end - origin + TILE - 1) / TILE;
+    const auto quad = [&](int i) {
+        if (i >= 0 && i <= p.vocab - 4)
+            return ld_stream16f(x + i);
+        float4 f = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+            const float y = i + c >= 0 && i + c < p.vocab ? __ldg(x + i + c) : -INFINITY;
+            f.x = c == 0 ? y : f.x, f.y = c == 1 ? y : f.y, f.z = c == 2 ? y : f.z, f.w = c == 3 ? y : f.w;
+        }
+        return f;
+    };
+    const auto load = [&](float4 (&v)[V], int tile) {
+        const int i = origin + tile * TILE + tid * 4;
+        if (i - tid * 4 >= 0 && i - tid * 4 + TILE <= p.vocab) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const float4 f = ld_stream16f(x + at + j * kLogprobThreads * 4);
-                v[j][0] = f.x, v[j][1] = f.y, v[j][2] = f.z, v[j][3] = f.w;
-            }
+            for (int j = 0; j < V; ++j)
+                v[j] = ld_stream16f(x + i + j * Q);
         } else {
-#pragma unroll
+#pragma unroll 1
             for (int j = 0; j < V; ++j) {
-                const int i = at + j * kLogprobThreads * 4;
-                if (i >= 0 && i <= p.vocab - 4) {
-                    const float4 f = ld_stream16f(x + i);
-                    v[j][0] = f.x, v[j][1] = f.y, v[j][2] = f.z, v[j][3] = f.w;
-                } else {
+                const float4 f = quad(i + j * Q);
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                        v[j][c] = i + c >= 0 && i + c < p.vocab ? __ldg(x + i + c) : -INFINITY;
-                }
+                for (int n = 0; n < V; ++n)
+                    v[n] = j == n ? f : v[n];
             }
         }
     };
-    float v[V][4];
-    load(v, base);
+    float4 va[V], vb[V];
+    load(va, 0);
     const float xt = token >= 0 && token < p.vocab ? __ldg(x + token) : INFINITY;  // outside: nothing in front
-    const float below = nextafterf(xt, -INFINITY);
-    float m = -INFINITY, r = 0.0f, e = 0.0f;  // r: 2^64 times the sum
+    // An id below the token is in front of it at an equal logit too: it is compared with the next value below. Below -inf
+    // there is none: of a masked token, all ids below it are in front (added after the loop) and those above it that are
+    // not masked. The four logits around the token have both kinds: put right after the loop.
+    const float below = xt == -INFINITY ? INFINITY : nextafterf(xt, -INFINITY);
+    float m = -INFINITY, r = 0.0f, e = 0.0f;  // r, e: 2^64 times the sums
     int before = 0;
-    float threshold = -INFINITY;
     if (tid == 0)
-        s_count = s_above = 0;
-    // The list's keys in order into s_top, at most top_k of them; 0 behind them.
-    const auto order = [&](int n) {
-        if (n <= kLogprobThreads) {  // a key's place is the number of larger ones
-            if (tid < n) {
-                const unsigned long long key = s_list[tid];
-                int place = 0;
-#pragma unroll 4
-                for (int i = 0; i < n; ++i)
-                    place += s_list[i] > key;
-                if (place < p.top_k)
-                    s_top[place] = key;
-            } else if (tid < p.top_k) {
-                s_top[tid] = 0ull;
+        s_count = s_threads = 0;
+    const auto work = [&](const float4 (&v)[V], int tile) {
+        float mine = fmaxf(fmaxf(v[0].x, v[0].y), fmaxf(v[0].z, v[0].w));
+#pragma unroll
+        for (int j = 1; j < V; ++j)
+            mine = fmaxf(fmaxf(mine, fmaxf(v[j].x, v[j].y)), fmaxf(v[j].z, v[j].w));
+        const float mn = fmaxf(m, mine), ms = mn == -INFINITY ? 0.0f : mn;
+        float tr = 0.0f, te = 0.0f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const float u0 = v[j].x - ms, u1 = v[j].y - ms, u2 = v[j].z - ms, u3 = v[j].w - ms;
+            const float w0 = weight_up(u0, p.inv_t), w1 = weight_up(u1, p.inv_t), w2 = weight_up(u2, p.inv_t),
+                        w3 = weight_up(u3, p.inv_t);
+            tr += (w0 + w1) + (w2 + w3);
+            te = fmaf(w0, fmaxf(u0, kLogprobLeast), te), te = fmaf(w1, fmaxf(u1, kLogprobLeast), te);
+            te = fmaf(w2, fmaxf(u2, kLogprobLeast), te), te = fmaf(w3, fmaxf(u3, kLogprobLeast), te);
+        }
+        // the sums so far, relative to the new largest (at 0 before the first logit above -inf)
+        const float u = fmaxf(m - ms, kLogprobLeast), w = weight_up(u, p.inv_t) * kLogprobDown;
+        e = w > 0.0f ? fmaf(w, fmaf(u, r, e), te) : te;  // u * r is finite where w is not 0
+        r = fmaf(w, r, tr);
+        m = mn;
+        if (mine >= xt) {
+            const int i = origin + tile * TILE + tid * 4;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float border = i + j * Q + 3 < token ? below : xt;
+                before += (v[j].x > border) + (v[j].y > border) + (v[j].z > border) + (v[j].w > border);
             }
-        } else {  // one by one
+        }
+    };
+#pragma unroll 1
+    for (int tile = 0; tile < tiles; tile += 2) {
+        if (tile + 1 < tiles)
+            load(vb, tile + 1);
+        work(va, tile);
+        if (tile + 1 < tiles) {
+            if (tile + 2 < tiles)
+                load(va, tile + 2);
+            work(vb, tile + 1);
+        }
+    }
+    if (tid == 0) {
+        if (token >= begin && token < end) {
+#pragma unroll 1
+            for (int i = max(token - ((token - origin) & 3), 0); i < token; ++i)
+                before += xt == -INFINITY ? -(__ldg(x + i) > xt) : __ldg(x + i) == xt;
+        }
+        if (xt == -INFINITY)
+            before += min(max(token - begin, 0), end - begin);
+    }
+
+    // The block's sums: every thread's relative to the largest.
+    float M = m;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+        M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    if (lane == 0)
+        s_m[warp] = M;
+    if (TOP)
+        s_mine[tid] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w)
+        M = fmaxf(M, s_m[w]);
+    {
+        const float u = fmaxf(m - (M == -INFINITY ? 0.0f : M), kLogprobLeast), w = weight_up(u, p.inv_t) * kLogprobDown;
+        e = w > 0.0f ? fmaf(u, r, e) * w : 0.0f;
+        r *= w;
+    }
+    const float own = r;
+    r = warp_sum(r);
+    e = warp_sum(e);
+    before = __reduce_add_sync(0xffffffffu, before);
+    if (lane == 0)
+        s_r[warp] = r, s_e[warp] = e, s_before[warp] = before;
+    if (TOP) {
+        // a thread's group of 4, a quarter of the groups each
+        const int mine = tid >> 2;
+        const auto group = [&](int g) {
+            return fmaxf(fmaxf(s_mine[4 * g], s_mine[4 * g + 1]), fmaxf(s_mine[4 * g + 2], s_mine[4 * g + 3]));
+        };
+        const float g = group(mine);
+        int place = 0;
+#pragma unroll 4
+        for (int k = 0; k < kLogprobGroups / 4; ++k) {
+            const int i = (tid & 3) + 4 * k;
+            const float h = group(i);
+            place += h > g || (h == g && i < mine);
+        }
+        place += __shfl_xor_sync(0xffffffffu, place, 1);
+        place += __shfl_xor_sync(0xffffffffu, place, 2);
+        if ((tid & 3) == 0 && place == p.top_k - 1)
+            s_threshold = g;
+    }
+    __syncthreads();
+    LogprobPiece sum{M, 0.0f, 0.0f, 0};
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w)
+        sum.r += s_r[w], sum.e += s_e[w], sum.before += s_before[w];
+    sum.r *= kLogprobDown;
+    sum.e *= kLogprobDown;
+    if (M == -INFINITY) {
+        sum.r = sum.r == sum.r ? 0.0f : NAN;
+        sum.e = 0.0f;
+    } else if (sum.r < 1.25f) {
+        // one logit is the largest, or the sum would be 2 or more: its thread's logits again, a float4 per lane
+        const unsigned holder = __ballot_sync(0xffffffffu, m == M);
+        __syncthreads();
+        if (holder) {
+            const int from = __ffs(holder) - 1, i0 = origin + (warp * 32 + from) * 4;
+            float rest = lane == from ? 0.0f : own;
+#pragma unroll 1
+            for (int q = lane; q < V * tiles; q += 32) {
+                const float4 f = quad(i0 + q / V * TILE + q % V * Q);
+                rest += f.x == M ? 0.0f : weight_up(f.x - M, p.inv_t);
+                rest += f.y == M ? 0.0f : weight_up(f.y - M, p.inv_t);
+                rest += f.z == M ? 0.0f : weight_up(f.z - M, p.inv_t);
+                rest += f.w == M ? 0.0f : weight_up(f.w - M, p.inv_t);
+            }
+            rest = warp_sum(rest);
+            if (lane == 0)
+                s_r[warp] = rest;
+        }
+        __syncthreads();
+        sum.r = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w)
+            sum.r += s_r[w];
+        sum.r *= kLogprobDown;
+    } else {
+        sum.r -= 1.0f;
+    }
+    // The keys of s_list[0, n) in order: the first top_k into s_top, 0 behind them. A key's place is the number of
+    // larger ones.
+    const auto order = [&](int n) {
+        if (tid < p.top_k)
+            s_top[tid] = 0ull;
+        __syncthreads();
+#pragma unroll 1
+        for (int k = tid; k < n; k += kLogprobThreads) {
+            const unsigned long long key = s_list[k];
+            int place = 0;
+#pragma unroll 8
+            for (int i = 0; i < n; ++i)
+                place += s_list[i] > key;
+            if (place < p.top_k && key)
+                s_top[place] = key;
+        }
+        __syncthreads();
+    };
+    if (TOP) {
+        const float threshold = s_threshold;
+        const bool masked = threshold == -INFINITY;  // then every logit above it is listed
+        if (masked ? m > threshold : m >= threshold)
+            s_thread[atomicAdd(&s_threads, 1)] = tid;
+        __syncthreads();
+        // Lists the logits of the threads at hand that reach the threshold, or lie above it.
+        const auto list = [&](bool above) {
+            const int items = s_threads * V * tiles;
+            const auto id_of = [&](int item) {
+                const int k = item / (V * tiles), q = item - k * V * tiles;
+                return origin + q / V * TILE + q % V * Q + s_thread[k] * 4;
+            };
+#pragma unroll 1
+            for (int item = tid; item < items; item += 3 * kLogprobThreads) {  // three loads under way
+                float4 f[3];
+#pragma unroll
+                for (int u = 0; u < 3; ++u)
+                    if (item + u * kLogprobThreads < items)
+                        f[u] = quad(id_of(item + u * kLogprobThreads));
+#pragma unroll 1
+                for (int u = 0; u < 3 && item + u * kLogprobThreads < items; ++u) {
+                    const float4 v = u == 0 ? f[0] : u == 1 ? f[1] : f[2];
+                    const float most = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
+                    if (above ? most <= threshold : most < threshold)
+                        continue;
+                    const int i = id_of(item + u * kLogprobThreads);
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        const float y = c == 0 ? v.x : c == 1 ? v.y : c == 2 ? v.z : v.w;
+                        if (above ? y > threshold : y >= threshold) {
+                            const int at = atomicAdd(&s_count, 1);
+                            if (at < kLogprobList)
+                                s_list[at] = order_key(y, i + c);
+                        }
+                    }
+                }
+            }
+        };
+        list(masked);
+        __syncthreads();
+        int n = s_count;
+        if (n > kLogprobList && !masked) {
+            __syncthreads();
+            if (tid == 0)
+                s_count = 0;
+            __syncthreads();
+            list(true);
+            if (warp == 0)
+                s_top[lane] = 0ull;
+            __syncthreads();
+            n = s_count;
+            if (n + kLogprobMaxTop <= kLogprobList) {
+                if (warp == 0) {
+                    const int id = logprob_equal_ids(x, threshold, begin, end, 0, p.top_k);
+                    s_list[n + lane] = id >= 0 ? order_key(threshold, id) : 0ull;
+                }
+                __syncthreads();
+                n += kLogprobMaxTop;
+            }
+        }
+        if (n <= kLogprobList) {
+            order(n);
+        } else {  // rows of many logits above it after all: one by one
             unsigned long long last = ~0ull;
 #pragma unroll 1
             for (int k = 0; k < p.top_k; ++k) {
                 unsigned long long next = 0ull;
-#pragma unroll 1
-                for (int i = tid; i < n; i += kLogprobThreads)
-                    next = s_list[i] < last && s_list[i] > next ? s_list[i] : next;
+#pragma unroll 4
+                for (int i = begin + tid; i < end; i += kLogprobThreads) {
+                    const float y = __ldg(x + i);
+                    const unsigned long long key = y > -INFINITY ? order_key(y, i) : 0ull;
+                    next = key < last && key > next ? key : next;
+                }
                 next = warp_max_key(next);
                 __syncthreads();
                 if (lane == 0)
@@ -201,255 +468,43 @@ __global__ void __launch_bounds__(kLogprobThreads, 4) k_logprob_pieces(LogprobDe
                 if (tid == 0)
                     s_top[k] = next;
             }
-        }
-        __syncthreads();
-    };
-    const auto id_of = [&](int bit) { return base + (bit >> 2) * kLogprobThreads * 4 + (bit & 3); };
-    const auto list = [&](unsigned bits, int at) {
-#pragma unroll 1
-        for (; bits; bits &= bits - 1, ++at) {
-            const int id = id_of(__ffs(bits) - 1);
-            s_list[at] = order_key(__ldg(x + id), id);
-        }
-    };
-    bool first_tile = true;
-#pragma unroll 1
-    for (;;) {
-        const int next = base + TILE;
-        float w4[V][4];
-        const bool more = next - tid * 4 < end;
-        if (more)
-            load(w4, next);
-        float mine = fmaxf(fmaxf(v[0][0], v[0][1]), fmaxf(v[0][2], v[0][3]));
-#pragma unroll
-        for (int j = 1; j < V; ++j)
-            mine = fmaxf(fmaxf(mine, fmaxf(v[j][0], v[j][1])), fmaxf(v[j][2], v[j][3]));
-        const float mn = fmaxf(m, mine), ms = mn == -INFINITY ? 0.0f : mn;
-        float tr = 0.0f, te = 0.0f;
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const float border = base + j * kLogprobThreads * 4 + 3 < token ? below : xt;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const float u = v[j][c] - ms, w = weight_up(u, p.inv_t);
-                tr += w;
-                te = fmaf(w, fmaxf(u, kLogprobLeast), te);
-                before += v[j][c] > border;
-            }
-        }
-        {  // the sums so far, relative to the new largest (at 0 before the first logit above -inf)
-            const float u = fmaxf(m - ms, kLogprobLeast), w = weight_up(u, p.inv_t) * kLogprobDown;
-            e = w > 0.0f ? fmaf(w, fmaf(u, r, e), te) : te;  // u * r is finite where w is not 0
-            r = fmaf(w, r, tr);
-            m = mn;
-        }
-        const int near = token - base;  // the token's place among the thread's: j * kLogprobThreads * 4 + c
-        if (xt == -INFINITY || ((unsigned)near < (unsigned)TILE && (near & (kLogprobThreads * 4 - 1)) < 4)) {
-            // nothing lies below -inf, and the four logits around the token have both kinds: counted one by one
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const int i = base + j * kLogprobThreads * 4;
-                const float border = i + 3 < token ? below : xt;
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    before += (v[j][c] > xt || (v[j][c] == xt && (unsigned)(i + c) < (unsigned)token)) - (v[j][c] > border);
-            }
-        }
-        if (p.top_k > 0) {
-            if (first_tile) {
-                float group = fmaxf(mine, __shfl_xor_sync(0xffffffffu, mine, 1));
-                group = fmaxf(group, __shfl_xor_sync(0xffffffffu, group, 2));
-                if ((tid & 3) == 0)
-                    s_group[tid >> 2] = group;
-                if (tid == 0)
-                    s_above = s_count;
-                __syncthreads();
-                if (tid < kLogprobGroups) {
-                    const float g = s_group[tid];
-                    int place = 0;
-#pragma unroll 8
-                    for (int i = 0; i < kLogprobGroups; ++i)
-                        place += s_group[i] > g || (s_group[i] == g && i < tid);
-                    if (place == p.top_k - 1)
-                        s_threshold = g;
-                }
-                __syncthreads();
-                threshold = s_threshold;
-            }
-            unsigned reach = 0;  // bit 4 j + c
-            if (first_tile ? mine >= threshold : mine > threshold) {
-#pragma unroll
-                for (int j = 0; j < V; ++j)
-#pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                        reach |= (first_tile ? v[j][c] >= threshold : v[j][c] > threshold) ? 1u << (4 * j + c) : 0u;
-                if (first_tile && threshold == -INFINITY) {  // keeps the row's ends out
-#pragma unroll 1
-                    for (int k = 0; k < 4 * V; ++k) {
-                        const int id = id_of(k);
-                        reach &= id >= 0 && id < p.vocab ? ~0u : ~(1u << k);
-                    }
-                }
-            }
-            const int at = reach ? atomicAdd(&s_count, __popc(reach)) : 0;
-            bool cut;
-            if (!first_tile) {
-                list(reach, at);
-                cut = __syncthreads_or(at + __popc(reach) > kLogprobKeep);
-            } else {
-                __syncthreads();
-                if (s_count <= kLogprobKeep) {
-                    list(reach, at);
-                } else {  // masses at the threshold
-                    unsigned equals = 0;
-                    if (reach) {
-#pragma unroll
-                        for (int j = 0; j < V; ++j)
-#pragma unroll
-                            for (int c = 0; c < 4; ++c)
-                                equals |= v[j][c] == threshold ? 1u << (4 * j + c) : 0u;
-                        equals &= reach;
-                    }
-                    const unsigned above = reach & ~equals;
-                    if (above)
-                        list(above, atomicAdd(&s_above, __popc(above)));
-                    __syncthreads();
-                    const int n = s_above;  // less than top_k carried, and less than top_k groups of threads
-                    int have = 0;
-#pragma unroll 1
-                    for (int j = 0; j < V && have < p.top_k; ++j) {  // by id: place j of every thread, then j + 1
-                        const unsigned bits = equals & (15u << (4 * j));
-                        int incl = __popc(bits);
-#pragma unroll
-                        for (int o = 1; o < 32; o <<= 1) {
-                            const int y = __shfl_up_sync(0xffffffffu, incl, o);
-                            if (lane >= o)
-                                incl += y;
-                        }
-                        if (lane == 31)
-                            s_ties[warp] = incl;
-                        __syncthreads();
-                        int to = have + incl - __popc(bits);
-#pragma unroll
-                        for (int w = 0; w < WARPS; ++w) {
-                            to += w < warp ? s_ties[w] : 0;
-                            have += s_ties[w];
-                        }
-#pragma unroll 1
-                        for (unsigned left = bits; left && to < p.top_k; left &= left - 1, ++to)
-                            s_list[n + to] = order_key(threshold, id_of(__ffs(left) - 1));
-                        __syncthreads();
-                    }
-                    if (tid == 0)
-                        s_count = n + min(have, p.top_k);
-                }
-                __syncthreads();
-                const int now = s_count;
-                __syncthreads();  // everyone has read it before the next tile adds
-                cut = now > kLogprobKeep;
-                first_tile = now < p.top_k;  // a row's ends, or NaN: the next tile fills the list up
-            }
-            if (cut) {
-                order(s_count);
-                if (tid < p.top_k)
-                    s_list[tid] = s_top[tid];
-                if (tid == 0)
-                    s_count = p.top_k;
-                threshold = key_logit(s_top[p.top_k - 1]);
-                __syncthreads();
-            }
-        }
-        base = next;
-        if (!more)
-            break;
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-                v[j][c] = w4[j][c];
-    }
-
-    // The block's sums: every thread's relative to the largest.
-    float M = m;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-        M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    if (lane == 0)
-        s_m[warp] = M;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w)
-        M = fmaxf(M, s_m[w]);
-    {
-        const float u = fmaxf(m - (M == -INFINITY ? 0.0f : M), kLogprobLeast), w = weight_up(u, p.inv_t) * kLogprobDown;
-        e = w > 0.0f ? fmaf(u, r, e) * w : 0.0f;
-        r *= w;
-    }
-    float mine_r = r;
-    r = warp_sum(r);
-    e = warp_sum(e);
-    before = __reduce_add_sync(0xffffffffu, before);
-    if (lane == 0)
-        s_r[warp] = r, s_e[warp] = e, s_before[warp] = before;
-    __syncthreads();
-    LogprobPiece sum{M, 0.0f, 0.0f, 0};
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w)
-        sum.r += s_r[w], sum.e += s_e[w], sum.before += s_before[w];
-    sum.r *= kLogprobDown;
-    sum.e *= kLogprobDown;
-    if (M > -INFINITY) {
-        if (sum.r < 1.25f) {
-            // Little beside the largest: its 1 has rounded the sum. The threads that hold a largest sum again,
-            // without them.
-            int equal = 0;
-            if (m == M) {
-                mine_r = 0.0f;
-#pragma unroll 1
-                for (int at = first + tid * 4; at - tid * 4 < end; at += TILE) {
-                    load(v, at);
-#pragma unroll
-                    for (int j = 0; j < V; ++j)
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            mine_r += v[j][c] == M ? 0.0f : weight_up(v[j][c] - M, p.inv_t);
-                            equal += v[j][c] == M;
-                        }
-                }
-            }
-            mine_r = warp_sum(mine_r);
-            equal = __reduce_add_sync(0xffffffffu, equal);
             __syncthreads();
-            if (lane == 0)
-                s_r[warp] = mine_r, s_equal[warp] = equal;
-            __syncthreads();
-            sum.r = 0.0f;
-            equal = 0;
-#pragma unroll
-            for (int w = 0; w < WARPS; ++w)
-                sum.r += s_r[w], equal += s_equal[w];
-            sum.r = fmaf(sum.r, kLogprobDown, (float)(equal - 1));
-        } else {
-            sum.r -= 1.0f;
         }
     }
-    if (p.top_k > 0)
-        order(s_count);
-    if (p.pieces == 1) {
-        const LogprobRow done(p, sum);
+    if (p.pieces > 1) {
+        if (!p.cluster) {
+            if (tid == 0)
+                stats[blockIdx.x] = sum;
+            if (TOP && tid < p.top_k)
+                tops[(size_t)blockIdx.x * p.top_k + tid] = s_top[tid];
+            return;
+        }
+        cg::cluster_group cluster = cg::this_cluster();
         if (tid == 0)
-            done.write(p, out, sum, row, token, xt);
-        if (tid < p.top_k)
-            done.write_top(out, (size_t)row * p.top_k + tid, s_top[tid]);
-        return;
+            s_sum = sum;
+        cluster.sync();
+        if (piece == 0) {
+            if (TOP && tid < p.pieces * p.top_k)  // at most 256 keys
+                s_list[tid] = cluster.map_shared_rank(s_top, tid / p.top_k)[tid % p.top_k];
+            if (warp == 0)
+                sum = logprob_join_sums(p, *cluster.map_shared_rank(&s_sum, min((unsigned)lane, (unsigned)p.pieces - 1)), p.pieces);
+        }
+        cluster.sync();  // the others' shared memory is read
+        if (piece > 0)
+            return;
+        if (TOP)
+            order(p.pieces * p.top_k);
     }
-    if (tid == 0)
-        stats[blockIdx.x] = sum;
-    if (tid < p.top_k)
-        tops[(size_t)blockIdx.x * p.top_k + tid] = s_top[tid];
+    if (warp == 0) {
+        const LogprobRow done(p, sum);
+        if (lane == 0)
+            done.write(p, out, sum, row, token, xt);
+        if (TOP)
+            done.write_top(p, out, row, lane < p.top_k ? s_top[lane] : 0ull, x);
+    }
 }
 
-// Joins a row's pieces: one CTA per row, a piece per thread at a time.
+// Joins a row's pieces where they are more than a cluster: one CTA per row, a piece per thread at a time.
 __global__ void __launch_bounds__(kLogprobJoinThreads) k_logprob_join(LogprobDev p, const float* __restrict__ logits,
                                                                       const int32_t* __restrict__ tokens,
                                                                       const LogprobPiece* __restrict__ stats,
@@ -509,30 +564,9 @@ __global__ void __launch_bounds__(kLogprobJoinThreads) k_logprob_join(LogprobDev
     if (p.top_k == 0)
         return;
     // The pieces' lists, each in order: the largest head top_k times.
-    if (p.pieces <= 32) {  // one warp: a list per lane, its next key at hand
-        if (warp > 0)
-            return;
-        const unsigned long long* list = tops + ((size_t)row * p.pieces + min(lane, p.pieces - 1)) * p.top_k;
-        unsigned long long head = lane < p.pieces ? list[0] : 0ull, mine_out = 0ull;
-        unsigned long long next = lane < p.pieces && p.top_k > 1 ? list[1] : 0ull;
-        int at = 2;
-#pragma unroll 1
-        for (int k = 0; k < p.top_k; ++k) {
-            const unsigned long long best = warp_max_key(head);
-            mine_out = k == lane ? best : mine_out;
-            if (head == best && best != 0ull) {  // keys differ: one lane
-                head = next;
-                next = at < p.top_k ? list[at] : 0ull;
-                ++at;
-            }
-        }
-        if (lane < p.top_k)
-            done.write_top(out, (size_t)row * p.top_k + lane, mine_out);
-        return;
-    }
     const unsigned long long* list = tops + (size_t)row * p.pieces * p.top_k;
     int at = 0;  // of the thread's first list
-    unsigned long long last = ~0ull, head = tid < p.pieces ? list[(size_t)tid * p.top_k] : 0ull;
+    unsigned long long last = ~0ull, head = tid < p.pieces ? list[(size_t)tid * p.top_k] : 0ull, mine_out = 0ull;
 #pragma unroll 1
     for (int k = 0; k < p.top_k; ++k) {
         unsigned long long best = head;
@@ -556,9 +590,10 @@ __global__ void __launch_bounds__(kLogprobJoinThreads) k_logprob_join(LogprobDev
             ++at;
             head = at < p.top_k ? list[(size_t)tid * p.top_k + at] : 0ull;
         }
-        if (tid == 0)
-            done.write_top(out, (size_t)row * p.top_k + k, best);
+        mine_out = tid == k ? best : mine_out;
     }
+    if (warp == 0)
+        done.write_top(p, out, row, mine_out, logits + row * p.stride);
 }
 
 }  // namespace muyo
@@ -578,15 +613,16 @@ static int logprobs_prepare(const MuyoTokenLogprobsParams* p, LogprobDev& d)
     d.stride = p->stride ? p->stride : p->vocab;
     d.temperature = p->temperature;
     d.inv_t = (float)(1.4426950408889634 / (double)p->temperature);
-    // Tiles of 4096 logits, of 2048 where the larger ones would leave SMs without a CTA; four CTAs on an SM at once, so a
-    // row is cut into the pieces that fill them. A row may begin 3 logits behind a 16-byte border.
-    const long long large = (d.vocab + 3LL + 4095) / 4096, room = 4LL * sm_count();
-    d.small = large * d.rows < sm_count();
-    const long long tiles = d.small ? (d.vocab + 3LL + 2047) / 2048 : large;
-    const long long cut = room / d.rows < 1 ? 1 : room / d.rows < tiles ? room / d.rows : tiles;
-    const long long each = (tiles + cut - 1) / cut;
-    d.tiles = (int)(each < kLogprobMaxTiles ? each : kLogprobMaxTiles);
-    d.pieces = (int)((tiles + d.tiles - 1) / d.tiles);
+    // Four CTAs on an SM at once: a row is cut into the pieces that fill them, and up to 8 of those are joined by
+    // their cluster. A row may begin 3 logits behind a 16-byte border.
+    const long long large = (d.vocab + 3LL + 16 * kLogprobThreads - 1) / (16 * kLogprobThreads), room = 4LL * sm_count() / d.rows;
+    d.small = large * d.rows < sm_count();  // the larger tiles would leave SMs without a CTA
+    const long long tiles = d.small ? (d.vocab + 3LL + 8 * kLogprobThreads - 1) / (8 * kLogprobThreads) : large;
+    const long long cut = std::max(1LL, std::min(room, tiles));
+    const long long each = std::min((tiles + cut - 1) / cut, (long long)kLogprobMaxTiles);
+    d.tiles = (int)each;
+    d.pieces = (int)((tiles + each - 1) / each);
+    d.cluster = d.pieces > 1 && d.pieces <= kLogprobCluster;
     if ((long long)d.pieces * d.rows > INT_MAX) {
         set_error("token_logprobs: %u rows of %u logits are more than 2^31 pieces", p->rows, p->vocab);
         return MUYO_EUNSUPPORTED;
@@ -623,11 +659,23 @@ extern "C" int muyo_cuda_token_logprobs(const MuyoTokenLogprobsParams* p, const 
     LogprobPiece* stats = static_cast<LogprobPiece*>(workspace);
     unsigned long long* tops = reinterpret_cast<unsigned long long*>(static_cast<char*>(workspace) + logprobs_stats_bytes(d));
     const LogprobOut o{logprob, entropy, rank, top_ids, top_logprobs};
-    const size_t smem = d.top_k ? (kLogprobKeep + (d.small ? 2048 : 4096)) * sizeof(unsigned long long) : 0;
-    MUYO_CUDA_TRY(launch_kernel(d.small ? k_logprob_pieces<2> : k_logprob_pieces<4>, dim3(d.rows * d.pieces),
-                                dim3(kLogprobThreads), smem, as_stream(stream), true, d, logits, tokens, stats, tops, o));
+    const auto kernel = d.small ? (d.top_k > 0 ? k_logprob_pieces<true, 2> : k_logprob_pieces<false, 2>)
+                                : (d.top_k > 0 ? k_logprob_pieces<true, 4> : k_logprob_pieces<false, 4>);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(d.rows * d.pieces);
+    cfg.blockDim = dim3(kLogprobThreads);
+    cfg.stream = as_stream(stream);
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)d.pieces;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = d.cluster ? 2 : 1;
+    MUYO_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, d, logits, tokens, stats, tops, o));
     MUYO_LAUNCH_CHECK();
-    if (d.pieces > 1) {
+    if (d.pieces > 1 && !d.cluster) {
         MUYO_CUDA_TRY(launch_kernel(k_logprob_join, dim3(d.rows), dim3(kLogprobJoinThreads), 0, as_stream(stream), true, d,
                                     logits, tokens, stats, tops, o));
         MUYO_LAUNCH_CHECK();
