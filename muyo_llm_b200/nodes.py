@@ -11,9 +11,10 @@ from . import _abi
 
 
 def _ptr(t) -> int | None:
-    if t is None:
-        return None
-    return t if isinstance(t, int) else t.data_ptr()
+    try:
+        return t.data_ptr()
+    except AttributeError:  # an address, or None
+        return t
 
 
 def _stream(s):
