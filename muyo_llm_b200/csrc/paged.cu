@@ -281,7 +281,7 @@ __device__ __forceinline__ void turn(float& a, float& b, double c, double s)
 constexpr int kAppendThreads = 256;
 
 template <typename KV, bool V4>
-__global__ void __launch_bounds__(kAppendThreads) k_paged_append(AppendDev p, const float* q, const float* k, const float* v,
+__global__ void __launch_bounds__(kAppendThreads, 4) k_paged_append(AppendDev p, const float* q, const float* k, const float* v,
                                                                  const int32_t* positions, const int32_t* slots,
                                                                  const double* __restrict__ freqs, float* q_out, KV* k_pool,
                                                                  KV* v_pool)
@@ -309,7 +309,7 @@ __global__ void __launch_bounds__(kAppendThreads) k_paged_append(AppendDev p, co
     if constexpr (V4) {
         const int per_head = hd / 8, turned = p.n_dims / 8;  // units
         const int qk = (heads + p.c.kv_heads) * per_head, all = qk + p.c.kv_heads * per_head;
-        constexpr int U = 4;  // a thread's units at a time
+        constexpr int U = 3;  // a thread's units at a time
         bool formed = false;
 #pragma unroll 1
         for (int base = tid; base - tid < all; base += U * kAppendThreads) {
