@@ -29,12 +29,15 @@
 // lane reads 16 contiguous bytes of a key's row for four (two) steps, and the keys of a step
 // are paired so that the scores' layout is the weights'. tcgen05 would hold 128 rows per tile for the 8 or 16 that one
 // token has; at these sizes the mma.sync issue is far below the memory time.
+#include <algorithm>
+
 #include "paged.cuh"
 
 namespace muyo {
 
-constexpr int kPagedWarps = 8;
+constexpr int kPagedWarps = 4;
 constexpr int kPagedThreads = 32 * kPagedWarps;
+constexpr int kPagedTile = 4096;  // bytes of a tile's keys
 
 struct PagedAttnDev {
     PagedDev c;
@@ -55,7 +58,7 @@ struct PagedTile {
     static constexpr int RB = HD * ES;        // bytes of a row
     static constexpr int CPR = RB / 16;       // 16-byte chunks of a row
     static constexpr int KSTEP = T == MUYO_KV_F32 ? 8 : 16;
-    static constexpr int KT = 4096 / RB > 64 ? 64 : 4096 / RB;  // keys of a tile
+    static constexpr int KT = kPagedTile / RB > 64 ? 64 : kPagedTile / RB < KSTEP ? KSTEP : kPagedTile / RB;  // keys of a tile
     static constexpr int STAGES = WIDE ? 2 : 3;
     static constexpr int TILE = KT * RB;      // bytes of a tile's keys (or values)
     static constexpr int ROWS = WIDE ? 16 : 8;
@@ -73,6 +76,7 @@ struct PagedTile {
     static_assert(KT % KSTEP == 0 && KT * CPR % 32 == 0, "tile shape");
     static_assert(RING >= PART * 4, "a drained ring holds a partial");
     static constexpr size_t SMEM = (size_t)kPagedWarps * (RING + PART * 4);
+    static constexpr int CTAS = SMEM <= 75 * 1024 ? 3 : 2;  // on an SM at once
 };
 
 template <int CPR>
@@ -137,17 +141,11 @@ __device__ __forceinline__ void split_half2(float a, float b, uint32_t& hi, uint
     lo = pack_half2(a - h.x, b - h.y);
 }
 
-__device__ __forceinline__ uint32_t tf32_rna(float x)
-{
-    uint32_t r;
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
-    return r;
-}
-
+// x as two TF32: its leading 11 bits and the next 11.
 __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo)
 {
-    hi = tf32_rna(x);
-    lo = tf32_rna(x - __uint_as_float(hi));
+    hi = __float_as_uint(x) & 0xffffe000u;
+    lo = __float_as_uint(x - __uint_as_float(hi)) & 0xffffe000u;
 }
 
 // Two e4m3 (the low 16 bits) as two F16, exactly.
@@ -227,7 +225,7 @@ struct PagedShares {
     }
 };
 
-// Pieces of one segment that a CTA joins: bit w the first piece of warp w, bit 8 + w its last one.
+// Pieces of one segment that a CTA joins: bit w the first piece of warp w, bit kPagedWarps + w its last one.
 struct PagedGroup {
     unsigned pieces;
     int seq, kv_head;
@@ -235,7 +233,7 @@ struct PagedGroup {
 };
 
 template <int T, int HD, bool WIDE>
-__global__ void __launch_bounds__(kPagedThreads, 1)
+__global__ void __launch_bounds__(kPagedThreads, (PagedTile<T, HD, WIDE>::CTAS))
 k_paged_attention(PagedAttnDev p, const float* __restrict__ q, const char* __restrict__ k_pool,
                   const char* __restrict__ v_pool, const int32_t* __restrict__ table, const int32_t* __restrict__ lens,
                   float* __restrict__ out, float* __restrict__ lse, float* __restrict__ part, PagedDesc* __restrict__ descs)
@@ -245,13 +243,21 @@ k_paged_attention(PagedAttnDev p, const float* __restrict__ q, const char* __res
     constexpr int W = kPagedWarps;
     extern __shared__ __align__(128) char paged_smem[];
     __shared__ unsigned long long s_mask[W][C::STAGES];
-    __shared__ int s_sum[W], s_start[W][2];
+    __shared__ int s_sum[W];
+    // the scan at first, the joins' rows and groups at the end (two CTAs' shared memory fits an SM to the byte)
+    union Shared {
+        int scan[kPagedThreads];
+        struct {
+            float2 rows[(W + 1) * C::ROWS];
+            PagedGroup group[W + 1];
+        } join;
+    };
+    __shared__ __align__(16) Shared s_u;
+    static_assert(kPagedThreads == 128, "four shares per lane");
     __shared__ int s_first[W], s_last[W];  // open pieces: 0 none, 1 open at the end, 2 ends here
     __shared__ int s_seg[W][4];            // request and KV head of the first and the last piece
     __shared__ int s_open;                 // tiles of the CTA's last segment behind its range
     __shared__ int s_groups;
-    __shared__ PagedGroup s_group[W + 1];
-    __shared__ float2 s_rows[(W + 1) * C::ROWS];
     pdl_wait();
     pdl_trigger();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -292,26 +298,7 @@ k_paged_attention(PagedAttnDev p, const float* __restrict__ q, const char* __res
     const PagedShares shares((unsigned)total, (unsigned)max(ctas, 1) * W);
     const int worker = blockIdx.x * W + warp;
     const bool idle = (int)blockIdx.x >= ctas;
-    if (!idle && mine > 0) {  // the warps whose first tile is of this thread's requests
-        const int excl = incl - mine;
-#pragma unroll 1
-        for (int w = 0; w < W; ++w) {
-            int rest = shares.begin(blockIdx.x * W + w) - excl;
-            if (rest < 0 || rest >= mine)
-                continue;
-            int s = s_begin;
-#pragma unroll 1
-            for (;; ++s) {
-                const PagedSpan<KT> span(p, __ldg(lens + s));
-                const int tiles = (span.t1 - span.t0) * p.c.kv_heads;
-                if (rest < tiles)
-                    break;
-                rest -= tiles;
-            }
-            s_start[w][0] = s;
-            s_start[w][1] = rest;
-        }
-    }
+    s_u.scan[tid] = incl;
     __syncthreads();
     if (empty) {  // requests without keys
 #pragma unroll 1
@@ -338,9 +325,20 @@ k_paged_attention(PagedAttnDev p, const float* __restrict__ q, const char* __res
     int left = u1 - shares.begin(worker), ahead = left;  // tiles to work on, to copy
     PagedCursor<KT> cur;
     if (left > 0) {
-        cur.s = s_start[warp][0];
-        cur.span = PagedSpan<KT>(p, __ldg(lens + cur.s));
-        const int tiles = cur.span.t1 - cur.span.t0, rest = s_start[warp][1];
+        // the first thread whose requests reach past the warp's first tile
+        const int u0 = u1 - left;
+        const int4 mark = *reinterpret_cast<const int4*>(&s_u.scan[4 * lane]);
+        const int share = __reduce_add_sync(0xffffffffu, (mark.x <= u0) + (mark.y <= u0) + (mark.z <= u0) + (mark.w <= u0));
+        int rest = u0 - (share > 0 ? s_u.scan[share - 1] : 0), tiles;
+        cur.s = share * per;
+#pragma unroll 1
+        for (;; ++cur.s) {
+            cur.span = PagedSpan<KT>(p, __ldg(lens + cur.s));
+            tiles = cur.span.t1 - cur.span.t0;
+            if (rest < tiles * p.c.kv_heads)
+                break;
+            rest -= tiles * p.c.kv_heads;
+        }
         cur.h = rest / tiles;
         cur.t = cur.span.t0 + rest - cur.h * tiles;
     }
@@ -428,16 +426,13 @@ k_paged_attention(PagedAttnDev p, const float* __restrict__ q, const char* __res
     uint32_t qf[NQ];              // fragments (F32 cache: q itself)
     float qs[HR], m[HR], l[HR];   // m: reference of the weights, the running maximum - 15
     float o[C::VPL][2 * HR];
-    bool fresh = true;            // a segment begins with the next tile
     bool whole = false;           // this warp has the segment from its first tile on
-    auto begin_segment = [&]() {
-        whole = cur.t == cur.span.t0;
+    float raw[HR][C::NKS * C::KPS];
+    auto load_q = [&]() {
         const float* qrow = q + cur.s * p.stride_q + (long long)cur.h * p.c.group * HD;
 #pragma unroll
         for (int r = 0; r < HR; ++r) {
             const int head = g + 8 * r;
-            float v[C::NKS * C::KPS];
-            float most = 0.0f;
 #pragma unroll
             for (int k = 0; k < C::NKS; ++k) {
                 constexpr int SPC = C::EPC / C::KPS;  // steps of a chunk
@@ -446,11 +441,21 @@ k_paged_attention(PagedAttnDev p, const float* __restrict__ q, const char* __res
                 for (int e = 0; e < C::KPS; e += 2) {
                     const float2 x = head < p.c.group ? __ldg(reinterpret_cast<const float2*>(qrow + head * HD + d + e))
                                                       : make_float2(0.0f, 0.0f);
-                    v[k * C::KPS + e] = x.x;
-                    v[k * C::KPS + e + 1] = x.y;
-                    most = fmaxf(most, fmaxf(fabsf(x.x), fabsf(x.y)));
+                    raw[r][k * C::KPS + e] = x.x;
+                    raw[r][k * C::KPS + e + 1] = x.y;
                 }
             }
+        }
+    };
+    auto begin_segment = [&]() {
+        whole = cur.t == cur.span.t0;
+#pragma unroll
+        for (int r = 0; r < HR; ++r) {
+            const float(&v)[C::NKS * C::KPS] = raw[r];
+            float most = 0.0f;
+#pragma unroll
+            for (int k = 0; k < C::NKS * C::KPS; ++k)
+                most = fmaxf(most, fabsf(v[k]));
             qs[r] = p.scale * 1.4426950408889634f;
             if constexpr (T == MUYO_KV_F32) {
 #pragma unroll
@@ -746,8 +751,10 @@ k_paged_attention(PagedAttnDev p, const float* __restrict__ q, const char* __res
     };
 
     if (left > 0) {
+        load_q();  // before the copies, which it would wait for
         look_up(true);
         int stage = 0, into = 0;
+        bool fresh = true;  // a segment begins with the next tile
 #pragma unroll 1
         for (int step = 1 - C::STAGES; left > 0; ++step) {
             if (ahead > 0)
@@ -765,7 +772,6 @@ k_paged_attention(PagedAttnDev p, const float* __restrict__ q, const char* __res
             stage = stage + 1 == C::STAGES ? 0 : stage + 1;
             --left;
             const bool ends = cur.t + 1 == cur.span.t1;
-            fresh = ends;
             if (ends || left == 0) {
                 if (!(whole && ends) && lane == 0) {
                     const int k = whole ? 2 : 0;
@@ -777,8 +783,12 @@ k_paged_attention(PagedAttnDev p, const float* __restrict__ q, const char* __res
                 // a piece that begins here and is open goes to the ring, which is drained then
                 end_segment(whole && ends ? nullptr : whole ? reinterpret_cast<float*>(ring) : first_part);
             }
-            if (left > 0)
+            fresh = ends;
+            if (left > 0) {
                 cur.next(p, lens);
+                if (ends)
+                    load_q();
+            }
         }
     }
     __syncthreads();
@@ -786,53 +796,55 @@ k_paged_attention(PagedAttnDev p, const float* __restrict__ q, const char* __res
     // ---- the CTA's join ----
     // A group is a piece that begins here (or comes in, to warp 0) and the first pieces of the warps behind it, up to the
     // one where the segment ends.
-    if (tid == 0) {
-        int groups = 0;
-        PagedDesc desc{0, 0, 0, 0};
-#pragma unroll 1
-        for (int k = -1; k < W; ++k) {  // -1: what comes in
-            const int w = max(k, 0);
-            if (k < 0 ? !s_first[0] : !s_last[w])
-                continue;
+    if (warp == 0) {
+        const int k = lane - 1, w = max(k, 0);  // lane 0: what comes in; lane w + 1: what begins in warp w
+        const bool is = lane <= W && (k < 0 ? s_first[0] != 0 : s_last[min(w, W - 1)] != 0);
+        const unsigned groups = __ballot_sync(0xffffffffu, is);
+        bool open = false;
+        if (is) {
             bool ended = k < 0 && s_first[0] == 2;
-            unsigned pieces = 1u << (k < 0 ? 0 : 8 + w);
-#pragma unroll 1
-            for (int v = w + 1; v < W && !ended; ++v) {
-                pieces |= s_first[v] ? 1u << v : 0u;
-                ended = s_first[v] == 2;
-            }
-            const PagedGroup group{pieces, s_seg[w][k < 0 ? 0 : 2], s_seg[w][k < 0 ? 1 : 3], k < 0 ? 0 : ended ? -1 : 1};
-            s_group[groups++] = group;
-            if (group.to == 1) {  // begun in this CTA and open behind it: one group at most
+            unsigned pieces = 1u << (k < 0 ? 0 : W + w);
+#pragma unroll
+            for (int v = 1; v < W; ++v)
+                if (v > w && !ended) {
+                    pieces |= s_first[v] ? 1u << v : 0u;
+                    ended = s_first[v] == 2;
+                }
+            open = k >= 0 && !ended;  // begun in this CTA and open behind it: one group at most
+            s_u.join.group[__popc(groups & ((1u << lane) - 1))] =
+                PagedGroup{pieces, s_seg[w][k < 0 ? 0 : 2], s_seg[w][k < 0 ? 1 : 3], k < 0 ? 0 : ended ? -1 : 1};
+            if (open) {
                 const int to = shares.worker_of((unsigned)(cta_end + s_open - 1)) / W;
-                desc = PagedDesc{group.seq, group.kv_head, to - (int)blockIdx.x + 1, 0};
+                descs[blockIdx.x] = PagedDesc{s_seg[w][2], s_seg[w][3], to - (int)blockIdx.x + 1, 0};
             }
         }
-        s_groups = groups;
-        descs[blockIdx.x] = desc;
+        if (!__any_sync(0xffffffffu, open) && lane == 0)
+            descs[blockIdx.x] = PagedDesc{0, 0, 0, 0};
+        if (lane == 0)
+            s_groups = __popc(groups);
     }
     __syncthreads();
     const int rows = s_groups * p.c.group;
-    // The pieces' weights 2^(m - M), in place of m, by 16 lanes per row; M and L by the group's first piece.
+    // The pieces' weights 2^(m - M), in place of m, by 2 W lanes per row; M and L by the first of them.
     auto piece_at = [&](int b) -> float* {
-        return reinterpret_cast<float*>(b < 8 ? paged_smem + (size_t)W * C::RING + (size_t)b * C::PART * 4
-                                              : paged_smem + (size_t)(b - 8) * C::RING);
+        return reinterpret_cast<float*>(b < W ? paged_smem + (size_t)W * C::RING + (size_t)b * C::PART * 4
+                                              : paged_smem + (size_t)(b - W) * C::RING);
     };
-    static_assert(W == 8, "a piece per lane of 16");
-    float* s_row = reinterpret_cast<float*>(s_rows);
+    constexpr int LANES = 2 * W;  // of a row
+    float* s_row = reinterpret_cast<float*>(s_u.join.rows);
 #pragma unroll 1
-    for (int i = tid >> 4; i < ((rows + 1) & ~1); i += kPagedThreads / 16) {
-        const int k = min(i, rows - 1) / p.c.group, r = min(i, rows - 1) % p.c.group, b = lane & 15;
-        const bool in = (s_group[k].pieces >> b) & 1;
+    for (int i = tid / LANES; i < (rows + 32 / LANES - 1) / (32 / LANES) * (32 / LANES); i += kPagedThreads / LANES) {
+        const int k = min(i, rows - 1) / p.c.group, r = min(i, rows - 1) % p.c.group, b = lane % LANES;
+        const bool in = (s_u.join.group[k].pieces >> b) & 1;
         float* at = piece_at(b) + C::ROWS * HD + r;
         float m1 = in ? at[0] : -INFINITY, l1 = in ? at[C::ROWS] : 0.0f, M = m1;
 #pragma unroll
-        for (int o2 = 8; o2 > 0; o2 >>= 1)
+        for (int o2 = LANES / 2; o2 > 0; o2 >>= 1)
             M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o2));
         const float w = l1 > 0.0f ? ex2(m1 - M) : 0.0f;
         float L = l1 * w;
 #pragma unroll
-        for (int o2 = 8; o2 > 0; o2 >>= 1)
+        for (int o2 = LANES / 2; o2 > 0; o2 >>= 1)
             L += __shfl_xor_sync(0xffffffffu, L, o2);
         if (i < rows) {
             if (in)
@@ -848,7 +860,7 @@ k_paged_attention(PagedAttnDev p, const float* __restrict__ q, const char* __res
     for (int i = tid; i < rows * (HD / 4); i += kPagedThreads) {
         const int row = i / (HD / 4), d = i % (HD / 4) * 4;
         const int k = row / p.c.group, r = row % p.c.group;
-        const PagedGroup group = s_group[k];
+        const PagedGroup group = s_u.join.group[k];
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 1
         for (unsigned bits = group.pieces; bits; bits &= bits - 1) {
@@ -877,7 +889,7 @@ k_paged_attention(PagedAttnDev p, const float* __restrict__ q, const char* __res
 // Joins the segment that begins in CTA blockIdx.x of the kernel above and ends in another: its last partial and the
 // first ones of the CTAs behind it. Four channels of a row per thread; threads to spare share the pieces.
 constexpr int kJoinThreads = 512;
-constexpr int kJoinPieces = 256;  // one per CTA at most
+constexpr int kJoinPieces = 480;  // one per CTA at most
 
 template <int HD, int ROWS>
 __global__ void __launch_bounds__(kJoinThreads) k_paged_join(PagedAttnDev p, const float* __restrict__ part,
@@ -974,18 +986,17 @@ static int paged_attention_prepare(const MuyoPagedAttentionParams* p, PagedAttnD
     return MUYO_OK;
 }
 
-// CTAs: one per SM, fewer when the tables could not hold a tile per warp.
-static int paged_attention_ctas(const PagedAttnDev& d)
+// CTAs at most: three per SM, fewer when the tables could not hold a tile per warp.
+static int paged_attention_ctas(const PagedAttnDev& d, int per_sm)
 {
     const long long tiles = ((long long)d.table_stride * d.c.page_size / 8 + 1) * d.c.kv_heads;
     const long long most = (tiles * d.seqs + kPagedWarps - 1) / kPagedWarps;
-    const int sms = sm_count() < kJoinPieces ? sm_count() : kJoinPieces;
-    return (int)(most < sms ? most : sms);
+    return (int)std::min({most, (long long)sm_count() * per_sm, (long long)kJoinPieces});
 }
 
 static size_t paged_attention_parts(const PagedAttnDev& d)
 {
-    return (size_t)paged_attention_ctas(d) * 2 * (d.c.group > 8 ? 16 : 8) * (d.c.head_dim + 2) * sizeof(float);
+    return (size_t)paged_attention_ctas(d, 3) * 2 * (d.c.group > 8 ? 16 : 8) * (d.c.head_dim + 2) * sizeof(float);
 }
 
 template <int T, int HD, bool WIDE>
@@ -995,7 +1006,7 @@ static int launch_paged_attention(const PagedAttnDev& d, const float* q, const v
     using C = PagedTile<T, HD, WIDE>;
     auto kernel = k_paged_attention<T, HD, WIDE>;
     MUYO_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM));
-    const int ctas = paged_attention_ctas(d);
+    const int ctas = paged_attention_ctas(d, C::CTAS);
     PagedAttnDev e = d;
     e.one_page = d.c.page_size % C::KT == 0;
     float* part = static_cast<float*>(ws);
@@ -1035,7 +1046,7 @@ extern "C" size_t muyo_cuda_paged_attention_workspace_size(const MuyoPagedAttent
     PagedAttnDev d{};
     if (!p || paged_attention_prepare(p, d) != MUYO_OK)
         return 0;
-    return paged_attention_parts(d) + (size_t)paged_attention_ctas(d) * sizeof(PagedDesc);
+    return paged_attention_parts(d) + (size_t)paged_attention_ctas(d, 3) * sizeof(PagedDesc);
 }
 
 extern "C" int muyo_cuda_paged_attention_decode(const MuyoPagedAttentionParams* p, const float* q, const void* k_pool,
