@@ -126,6 +126,40 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], 
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// The first product of a sum: from zero.
+__device__ __forceinline__ void mma_f16_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
+__device__ __forceinline__ void mma_tf32_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
+// Pairs of F32: a + b, and a * b + c.
+__device__ __forceinline__ float2 add2(float2 a, float2 b)
+{
+    float2 r;
+    asm("{.reg .b64 x, y; mov.b64 x, {%2,%3}; mov.b64 y, {%4,%5}; add.rn.f32x2 x, x, y; mov.b64 {%0,%1}, x;}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
+{
+    float2 r;
+    asm("{.reg .b64 x, y, z; mov.b64 x, {%2,%3}; mov.b64 y, {%4,%5}; mov.b64 z, {%6,%7}; fma.rn.f32x2 x, x, y, z; "
+        "mov.b64 {%0,%1}, x;}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
+}
+
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi)
 {
     uint32_t r;
@@ -388,13 +422,24 @@ k_paged_attention(PagedAttnDev p, const float* __restrict__ q, const char* __res
             for (int i = 0; i < (KT + 31) / 32; ++i)
                 mask |= (unsigned long long)__ballot_sync(0xffffffffu, i * 32 + lane >= lo && i * 32 + lane < min(hi, KT))
                         << (32 * i);
+            const char *kp = k_pool + o, *vp = v_pool + o;
+            if (lo <= 0 && hi >= KT) {
 #pragma unroll
+                for (int i = 0; i < KT * C::CPR / 32; ++i) {
+                    const int row = i * RPI + row0;
+                    copy16(kd + row * C::RB + k_chunk<C::CPR>(row, ch) * 16, kp, true);
+                    copy16(vd + row * C::RB + v_chunk<C::CPR>(row, ch) * 16, vp, true);
+                    kp += RPI * slot_bytes, vp += RPI * slot_bytes;
+                }
+            } else {
+#pragma unroll 1
             for (int i = 0; i < KT * C::CPR / 32; ++i) {
                 const int row = i * RPI + row0;
                 const bool seen = row >= lo && row < hi;
-                copy16(kd + row * C::RB + k_chunk<C::CPR>(row, ch) * 16, k_pool + (seen ? o : 0), seen);
-                copy16(vd + row * C::RB + v_chunk<C::CPR>(row, ch) * 16, v_pool + (seen ? o : 0), seen);
-                o += RPI * slot_bytes;
+                copy16(kd + row * C::RB + k_chunk<C::CPR>(row, ch) * 16, seen ? kp : k_pool, seen);
+                copy16(vd + row * C::RB + v_chunk<C::CPR>(row, ch) * 16, seen ? vp : v_pool, seen);
+                kp += RPI * slot_bytes, vp += RPI * slot_bytes;
+            }
             }
         } else {
             long long off[(KT + 31) / 32];
@@ -492,6 +537,16 @@ k_paged_attention(PagedAttnDev p, const float* __restrict__ q, const char* __res
                 o[n][e] = 0.0f;
     };
 
+    // A tile's products into the running sums: the two halves' rows added up, or a row's sums of each head.
+    const auto add_tile = [](float(&on)[2 * HR], const float(&alpha)[HR], const float(&acc)[4]) {
+        const float2 upper = make_float2(acc[0], acc[1]), lower = make_float2(acc[2], acc[3]);
+        const float2 first = fma2(make_float2(on[0], on[1]), make_float2(alpha[0], alpha[0]), WIDE ? upper : add2(upper, lower));
+        on[0] = first.x, on[1] = first.y;
+        if constexpr (WIDE) {
+            const float2 second = fma2(make_float2(on[2], on[3]), make_float2(alpha[1], alpha[1]), lower);
+            on[2] = second.x, on[3] = second.y;
+        }
+    };
     auto tile = [&](int stage) {
         const uint32_t ks = ring_at + stage * 2 * C::TILE, vs = ks + C::TILE;
         const unsigned long long mask = s_mask[warp][stage];
@@ -499,7 +554,7 @@ k_paged_attention(PagedAttnDev p, const float* __restrict__ q, const char* __res
         float s[KT / 8][2 * HR];
 #pragma unroll
         for (int j = 0; j < KT / 8; ++j) {
-            float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            float acc[4], small[4];  // small: an F32 cache's products with the remainders
             const int row = j * 8 + g;
 #pragma unroll
             for (int i = 0; i < C::NCH; ++i) {
@@ -520,13 +575,13 @@ k_paged_attention(PagedAttnDev p, const float* __restrict__ q, const char* __res
                                 split_tf32(__uint_as_float(qf[(k * 2 + e) * HR + r]), ah[2 * e + r], al[2 * e + r]);
                         }
                         if constexpr (WIDE) {
-                            mma_tf32(acc, al, bh[0], bh[1]);
-                            mma_tf32(acc, ah, bl[0], bl[1]);
-                            mma_tf32(acc, ah, bh[0], bh[1]);
+                            k == 0 ? mma_tf32_first(small, al, bh[0], bh[1]) : mma_tf32(small, al, bh[0], bh[1]);
+                            mma_tf32(small, ah, bl[0], bl[1]);
+                            k == 0 ? mma_tf32_first(acc, ah, bh[0], bh[1]) : mma_tf32(acc, ah, bh[0], bh[1]);
                         } else {
                             const uint32_t a[4] = {ah[0], al[0], ah[2], al[2]};
-                            mma_tf32(acc, a, bl[0], bl[1]);
-                            mma_tf32(acc, a, bh[0], bh[1]);
+                            k == 0 ? mma_tf32_first(small, a, bl[0], bl[1]) : mma_tf32(small, a, bl[0], bl[1]);
+                            k == 0 ? mma_tf32_first(acc, a, bh[0], bh[1]) : mma_tf32(acc, a, bh[0], bh[1]);
                         }
                     } else {
                         uint32_t b0, b1;
@@ -538,14 +593,19 @@ k_paged_attention(PagedAttnDev p, const float* __restrict__ q, const char* __res
                         if constexpr (WIDE) {
                             const uint32_t lo[4] = {qf[k * 8 + 4], qf[k * 8 + 5], qf[k * 8 + 6], qf[k * 8 + 7]};
                             const uint32_t hi[4] = {qf[k * 8], qf[k * 8 + 1], qf[k * 8 + 2], qf[k * 8 + 3]};
-                            mma_f16(acc, lo, b0, b1);
+                            k == 0 ? mma_f16_first(acc, lo, b0, b1) : mma_f16(acc, lo, b0, b1);
                             mma_f16(acc, hi, b0, b1);
                         } else {
                             const uint32_t a[4] = {qf[k * 4], qf[k * 4 + 1], qf[k * 4 + 2], qf[k * 4 + 3]};
-                            mma_f16(acc, a, b0, b1);
+                            k == 0 ? mma_f16_first(acc, a, b0, b1) : mma_f16(acc, a, b0, b1);
                         }
                     }
                 }
+            }
+            if constexpr (T == MUYO_KV_F32) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    acc[e] += small[e];
             }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
@@ -615,7 +675,7 @@ k_paged_attention(PagedAttnDev p, const float* __restrict__ q, const char* __res
                     }
 #pragma unroll
                 for (int n = 0; n < C::VE; ++n) {
-                    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    float acc[4];
 #pragma unroll
                     for (int j = 0; j < KT / 8; ++j) {
                         uint32_t bh[2], bl[2];
@@ -623,25 +683,17 @@ k_paged_attention(PagedAttnDev p, const float* __restrict__ q, const char* __res
                         for (int e = 0; e < 2; ++e)
                             split_tf32(__uint_as_float(v[j][e].w[n]), bh[e], bl[e]);
                         if constexpr (WIDE) {
-                            mma_tf32(acc, wl[j], bh[0], bh[1]);
+                            j == 0 ? mma_tf32_first(acc, wl[j], bh[0], bh[1]) : mma_tf32(acc, wl[j], bh[0], bh[1]);
                             mma_tf32(acc, wh[j], bl[0], bl[1]);
                             mma_tf32(acc, wh[j], bh[0], bh[1]);
                         } else {
                             const uint32_t a[4] = {wh[j][0], wl[j][0], wh[j][2], wl[j][2]};
-                            mma_tf32(acc, a, bl[0], bl[1]);
+                            j == 0 ? mma_tf32_first(acc, a, bl[0], bl[1]) : mma_tf32(acc, a, bl[0], bl[1]);
                             mma_tf32(acc, a, bh[0], bh[1]);
                         }
                     }
                     float(&on)[2 * HR] = o[ic * C::VE + n];
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        if constexpr (WIDE) {
-                            on[e] = fmaf(on[e], alpha[0], acc[e]);
-                            on[2 + e] = fmaf(on[2 + e], alpha[1], acc[2 + e]);
-                        } else {
-                            on[e] = fmaf(on[e], alpha[0], acc[e] + acc[2 + e]);
-                        }
-                    }
+                    add_tile(on, alpha, acc);
                 }
             }
         } else {
@@ -671,7 +723,7 @@ k_paged_attention(PagedAttnDev p, const float* __restrict__ q, const char* __res
                     }
 #pragma unroll
                 for (int n = 0; n < C::VE; ++n) {
-                    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    float acc[4];
 #pragma unroll
                     for (int j = 0; j < KT / 16; ++j) {
                         uint32_t b[2];
@@ -687,23 +739,15 @@ k_paged_attention(PagedAttnDev p, const float* __restrict__ q, const char* __res
                         if constexpr (WIDE) {
                             const uint32_t lo[4] = {w[j][4], w[j][5], w[j][6], w[j][7]};
                             const uint32_t hi[4] = {w[j][0], w[j][1], w[j][2], w[j][3]};
-                            mma_f16(acc, lo, b[0], b[1]);
+                            j == 0 ? mma_f16_first(acc, lo, b[0], b[1]) : mma_f16(acc, lo, b[0], b[1]);
                             mma_f16(acc, hi, b[0], b[1]);
                         } else {
                             const uint32_t a[4] = {w[j][0], w[j][1], w[j][2], w[j][3]};
-                            mma_f16(acc, a, b[0], b[1]);
+                            j == 0 ? mma_f16_first(acc, a, b[0], b[1]) : mma_f16(acc, a, b[0], b[1]);
                         }
                     }
                     float(&on)[2 * HR] = o[ic * C::VE + n];
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        if constexpr (WIDE) {
-                            on[e] = fmaf(on[e], alpha[0], acc[e]);
-                            on[2 + e] = fmaf(on[2 + e], alpha[1], acc[2 + e]);
-                        } else {
-                            on[e] = fmaf(on[e], alpha[0], acc[e] + acc[2 + e]);
-                        }
-                    }
+                    add_tile(on, alpha, acc);
                 }
             }
         }
