@@ -554,7 +554,9 @@ k_paged_attention(PagedAttnDev p, const float* __restrict__ q, const char* __res
         float s[KT / 8][2 * HR];
 #pragma unroll
         for (int j = 0; j < KT / 8; ++j) {
-            float acc[4], small[4];  // small: an F32 cache's products with the remainders
+            // An F32 cache's steps in turns by two sums, the products with the remainders apart: short chains.
+            constexpr int S = T == MUYO_KV_F32 && C::NKS > 2 ? 2 : 1;
+            float acc[4], accs[S][4], less[S][4], least[S][4];
             const int row = j * 8 + g;
 #pragma unroll
             for (int i = 0; i < C::NCH; ++i) {
@@ -575,13 +577,13 @@ k_paged_attention(PagedAttnDev p, const float* __restrict__ q, const char* __res
                                 split_tf32(__uint_as_float(qf[(k * 2 + e) * HR + r]), ah[2 * e + r], al[2 * e + r]);
                         }
                         if constexpr (WIDE) {
-                            k == 0 ? mma_tf32_first(small, al, bh[0], bh[1]) : mma_tf32(small, al, bh[0], bh[1]);
-                            mma_tf32(small, ah, bl[0], bl[1]);
-                            k == 0 ? mma_tf32_first(acc, ah, bh[0], bh[1]) : mma_tf32(acc, ah, bh[0], bh[1]);
+                            k < S ? mma_tf32_first(less[k % S], al, bh[0], bh[1]) : mma_tf32(less[k % S], al, bh[0], bh[1]);
+                            k < S ? mma_tf32_first(least[k % S], ah, bl[0], bl[1]) : mma_tf32(least[k % S], ah, bl[0], bl[1]);
+                            k < S ? mma_tf32_first(accs[k % S], ah, bh[0], bh[1]) : mma_tf32(accs[k % S], ah, bh[0], bh[1]);
                         } else {
                             const uint32_t a[4] = {ah[0], al[0], ah[2], al[2]};
-                            k == 0 ? mma_tf32_first(small, a, bl[0], bl[1]) : mma_tf32(small, a, bl[0], bl[1]);
-                            k == 0 ? mma_tf32_first(acc, a, bh[0], bh[1]) : mma_tf32(acc, a, bh[0], bh[1]);
+                            k < S ? mma_tf32_first(less[k % S], a, bl[0], bl[1]) : mma_tf32(less[k % S], a, bl[0], bl[1]);
+                            k < S ? mma_tf32_first(accs[k % S], a, bh[0], bh[1]) : mma_tf32(accs[k % S], a, bh[0], bh[1]);
                         }
                     } else {
                         uint32_t b0, b1;
@@ -604,8 +606,18 @@ k_paged_attention(PagedAttnDev p, const float* __restrict__ q, const char* __res
             }
             if constexpr (T == MUYO_KV_F32) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    acc[e] += small[e];
+                for (int e = 0; e < 4; ++e) {
+                    float low = less[0][e];
+                    acc[e] = accs[0][e];
+                    if constexpr (S > 1)
+                        low += less[1][e], acc[e] += accs[1][e];
+                    if constexpr (WIDE) {
+                        low += least[0][e];
+                        if constexpr (S > 1)
+                            low += least[1][e];
+                    }
+                    acc[e] += low;
+                }
             }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
