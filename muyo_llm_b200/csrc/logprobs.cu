@@ -390,36 +390,38 @@ __global__ void __launch_bounds__(kLogprobThreads, 4) k_logprob_pieces(LogprobDe
         __syncthreads();
         // Lists the logits of the threads at hand that reach the threshold, or lie above it.
         const auto list = [&](bool above) {
-            const int items = s_threads * V * tiles;
-            const auto id_of = [&](int item) {
-                const int k = item / (V * tiles), q = item - k * V * tiles;
-                return origin + q / V * TILE + q % V * Q + s_thread[k] * 4;
-            };
+            // a warp reads four threads' logits at once, a float4 of each per lane
+            const int threads = s_threads;
 #pragma unroll 1
-            for (int item = tid; item < items; item += 3 * kLogprobThreads) {  // three loads under way
-                float4 f[3];
+            for (int k0 = warp; k0 < threads; k0 += 4 * WARPS)
+#pragma unroll 1
+                for (int q = lane; q < V * tiles; q += 32) {
+                    float4 f[4];
+                    int id[4];
 #pragma unroll
-                for (int u = 0; u < 3; ++u)
-                    if (item + u * kLogprobThreads < items)
-                        f[u] = quad(id_of(item + u * kLogprobThreads));
+                    for (int u = 0; u < 4; ++u) {
+                        f[u].x = f[u].y = f[u].z = f[u].w = -INFINITY;
+                        if (k0 + u * WARPS < threads) {
+                            id[u] = origin + q / V * TILE + q % V * Q + s_thread[k0 + u * WARPS] * 4;
+                            f[u] = quad(id[u]);
+                        }
+                    }
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const float most = fmaxf(fmaxf(f[u].x, f[u].y), fmaxf(f[u].z, f[u].w));
+                        if (k0 + u * WARPS >= threads || (above ? most <= threshold : most < threshold))
+                            continue;
 #pragma unroll 1
-                for (int u = 0; u < 3 && item + u * kLogprobThreads < items; ++u) {
-                    const float4 v = u == 0 ? f[0] : u == 1 ? f[1] : f[2];
-                    const float most = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
-                    if (above ? most <= threshold : most < threshold)
-                        continue;
-                    const int i = id_of(item + u * kLogprobThreads);
-#pragma unroll 1
-                    for (int c = 0; c < 4; ++c) {
-                        const float y = c == 0 ? v.x : c == 1 ? v.y : c == 2 ? v.z : v.w;
-                        if (above ? y > threshold : y >= threshold) {
-                            const int at = atomicAdd(&s_count, 1);
-                            if (at < kLogprobList)
-                                s_list[at] = order_key(y, i + c);
+                        for (int c = 0; c < 4; ++c) {
+                            const float y = c == 0 ? f[u].x : c == 1 ? f[u].y : c == 2 ? f[u].z : f[u].w;
+                            if (above ? y > threshold : y >= threshold) {
+                                const int at = atomicAdd(&s_count, 1);
+                                if (at < kLogprobList)
+                                    s_list[at] = order_key(y, id[u] + c);
+                            }
                         }
                     }
                 }
-            }
         };
         list(masked);
         __syncthreads();
@@ -613,12 +615,16 @@ static int logprobs_prepare(const MuyoTokenLogprobsParams* p, LogprobDev& d)
     d.stride = p->stride ? p->stride : p->vocab;
     d.temperature = p->temperature;
     d.inv_t = (float)(1.4426950408889634 / (double)p->temperature);
-    // Four CTAs on an SM at once: a row is cut into the pieces that fill them, and up to 8 of those are joined by
-    // their cluster. A row may begin 3 logits behind a 16-byte border.
-    const long long large = (d.vocab + 3LL + 16 * kLogprobThreads - 1) / (16 * kLogprobThreads), room = 4LL * sm_count() / d.rows;
+    // A row is cut into the pieces that come nearest to three CTAs on an SM (97 rows of 151936 with 20 alternatives: 5
+    // pieces 23.5 us, 6 pieces 30 us, the ends of more pieces cost more than their loops gain; 150 rows: 2 pieces 44
+    // us, 3 pieces 34 us), and not into more than a cluster joins where those are a CTA per SM (40 rows: 8 pieces 20
+    // us, 14 pieces and a second kernel 22 us; one row: 8 pieces 13 us, 75 pieces 8 us). A row may begin 3 logits behind a 16-byte border.
+    const long long large = (d.vocab + 3LL + 16 * kLogprobThreads - 1) / (16 * kLogprobThreads);
     d.small = large * d.rows < sm_count();  // the larger tiles would leave SMs without a CTA
     const long long tiles = d.small ? (d.vocab + 3LL + 8 * kLogprobThreads - 1) / (8 * kLogprobThreads) : large;
-    const long long cut = std::max(1LL, std::min(room, tiles));
+    long long cut = std::max(1LL, std::min((3LL * sm_count() + d.rows / 2) / d.rows, tiles));
+    if (cut > kLogprobCluster && d.rows * (long long)kLogprobCluster >= sm_count())
+        cut = kLogprobCluster;
     const long long each = std::min((tiles + cut - 1) / cut, (long long)kLogprobMaxTiles);
     d.tiles = (int)each;
     d.pieces = (int)((tiles + each - 1) / each);

@@ -24,6 +24,7 @@ constexpr unsigned kPlanAdmitted = 0x80000000u, kPlanEnded = 0x40000000u, kPlanH
 
 struct PlanDev {
     int seqs, page_size, num_pages, table_stride, max_tokens;
+    int page_shift;  // log2(page_size), or -1
 };
 
 struct PlanSums {
@@ -57,10 +58,16 @@ __device__ __forceinline__ int first_above(const int* sums, int n, int x)
     return lo;
 }
 
-__device__ __forceinline__ int ring_index(long long i, int n)
+// Entry `by` places behind entry `from` of a ring of n (from < n, by <= n).
+__device__ __forceinline__ int ring_index(int from, int by, int n)
 {
-    const long long r = i % n;
-    return (int)(r < 0 ? r + n : r);
+    const unsigned r = (unsigned)from + (unsigned)by;
+    return (int)(r < (unsigned)n ? r : r - (unsigned)n);
+}
+
+__device__ __forceinline__ int page_of(const PlanDev& p, int slot)
+{
+    return p.page_shift >= 0 ? slot >> p.page_shift : slot / p.page_size;
 }
 
 __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads) k_paged_plan(PlanDev p, const int32_t* cached_lens, const int32_t* new_lens,
@@ -91,10 +98,10 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
     PlanSums mine{0, 0, 0};
     for (int i = i0; i < i1; ++i) {
         const int c = min(max(cached_lens[i], 0), row_slots), n = new_lens[i];
-        const int had = (c + p.page_size - 1) / p.page_size;
+        const int had = page_of(p, c + p.page_size - 1);
         const bool fits = n > 0 && n <= row_slots - c;
         mine.tokens += max(n, 0);
-        mine.pages += fits ? (c + n - 1) / p.page_size + 1 - had : 0;
+        mine.pages += fits ? page_of(p, c + n - 1) + 1 - had : 0;
         mine.ended += n < 0 ? had : 0;
     }
     PlanSums incl = mine;
@@ -125,10 +132,10 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
     int taken = 0, refused = 0;
     for (int i = i0; i < i1; ++i) {
         const int c = min(max(cached_lens[i], 0), row_slots), n = new_lens[i];
-        const int had = (c + p.page_size - 1) / p.page_size;
+        const int had = page_of(p, c + p.page_size - 1);
         const bool fits = n > 0 && n <= row_slots - c;
         run.tokens += max(n, 0);
-        run.pages += fits ? (c + n - 1) / p.page_size + 1 - had : 0;
+        run.pages += fits ? page_of(p, c + n - 1) + 1 - had : 0;
         run.ended += n < 0 ? had : 0;
         const bool ok = fits && run.pages <= free_pages && run.tokens <= p.max_tokens;
         stop[i] = saturated(run.tokens);
@@ -145,6 +152,11 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
         atomicAdd(&s_refused, refused);
     cg::this_cluster().sync();  // every CTA has read the lengths and the state
     taken = s_taken;
+    const auto place = [&](long long i) {
+        const long long r = i % p.num_pages;
+        return (int)(r < 0 ? r + p.num_pages : r);
+    };
+    const int first = place(head), last = place(tail);
     const int back = (int)min(total.ended, (long long)(p.num_pages - free_pages));
     // requests
     for (int i = all; i < p.seqs; i += kPlanCtas * kPlanThreads) {
@@ -159,13 +171,13 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
         int slot = -1, pos = 0;
         if (i < p.seqs && (held[i] & kPlanAdmitted)) {
             const int c = (int)(held[i] & kPlanHeld);
-            const int had = (c + p.page_size - 1) / p.page_size;
+            const int had = page_of(p, c + p.page_size - 1);
             pos = c + t - (i > 0 ? stop[i - 1] : 0);
-            const int at = pos / p.page_size;
+            const int at = page_of(p, pos);
             const int page = at < had ? table[(size_t)i * p.table_stride + at]
-                                      : ring[ring_index(head + (i > 0 ? upto[i - 1] : 0) + (at - had), p.num_pages)];
+                                      : ring[ring_index(first, (i > 0 ? upto[i - 1] : 0) + (at - had), p.num_pages)];
             if (page >= 0 && page < p.num_pages)
-                slot = page * p.page_size + pos % p.page_size;
+                slot = page * p.page_size + pos - at * p.page_size;
         }
         slots[t] = slot;
         positions[t] = pos;
@@ -173,13 +185,13 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
     // pages from the ring into the tables
     for (int k = all; k < taken; k += kPlanCtas * kPlanThreads) {
         const int i = first_above(upto, p.seqs, k);
-        const int had = ((int)(held[i] & kPlanHeld) + p.page_size - 1) / p.page_size;
-        table[(size_t)i * p.table_stride + had + k - (i > 0 ? upto[i - 1] : 0)] = ring[ring_index(head + k, p.num_pages)];
+        const int had = page_of(p, (int)(held[i] & kPlanHeld) + p.page_size - 1);
+        table[(size_t)i * p.table_stride + had + k - (i > 0 ? upto[i - 1] : 0)] = ring[ring_index(first, k, p.num_pages)];
     }
     // pages of ended requests into the ring
     for (int k = all; k < back; k += kPlanCtas * kPlanThreads) {
         const int i = first_above(gone, p.seqs, k);
-        ring[ring_index(tail + k, p.num_pages)] = table[(size_t)i * p.table_stride + k - (i > 0 ? gone[i - 1] : 0)];
+        ring[ring_index(last, k, p.num_pages)] = table[(size_t)i * p.table_stride + k - (i > 0 ? gone[i - 1] : 0)];
     }
     if (all == 0) {
         query_start[p.seqs] = saturated(total.tokens);
@@ -441,7 +453,8 @@ extern "C" int muyo_cuda_paged_plan(const MuyoPagedPlanParams* p, const int32_t*
                  "paged_plan: null buffer");
     MUYO_REQUIRE(p->max_tokens == 0 || (positions && slots), "paged_plan: positions and slots are needed with max_tokens");
     MUYO_REQUIRE(aligned_to(state, 8) && aligned_to(state_out, 8), "paged_plan: state must be 8-byte aligned");
-    const PlanDev d{(int)p->seqs, (int)p->page_size, (int)p->num_pages, (int)p->table_stride, (int)p->max_tokens};
+    const PlanDev d{(int)p->seqs, (int)p->page_size, (int)p->num_pages, (int)p->table_stride, (int)p->max_tokens,
+                    page_shift_of((int)p->page_size)};
     const size_t smem = (size_t)p->seqs * 4 * sizeof(int);
     if (smem > 48 * 1024)
         MUYO_CUDA_TRY(cudaFuncSetAttribute(k_paged_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));

@@ -56,6 +56,15 @@ inline int paged_prepare(const MuyoPagedCache& c, const char* what, PagedDev& d)
     return MUYO_OK;
 }
 
+// log2 of a power of two, or -1.
+inline int page_shift_of(int page_size)
+{
+    for (int s = 0; s < 31; ++s)
+        if (page_size == 1 << s)
+            return s;
+    return -1;
+}
+
 inline bool aligned_to(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
 }  // namespace muyo

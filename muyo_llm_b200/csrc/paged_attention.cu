@@ -1035,10 +1035,7 @@ static int paged_attention_prepare(const MuyoPagedAttentionParams* p, PagedAttnD
     }
     d.seqs = (int)p->seqs, d.table_stride = (int)p->table_stride, d.window = (int)p->window;
     d.scale = p->scale * d.c.k_scale;
-    d.page_shift = -1;
-    for (int s = 0; s < 31; ++s)
-        if (d.c.page_size == 1 << s)
-            d.page_shift = s;
+    d.page_shift = page_shift_of(d.c.page_size);
     return MUYO_OK;
 }
 
