@@ -461,6 +461,7 @@ int muyo_p2p_destroy(MuyoP2PGroup* g);
  * A step is one muyo_cuda_paged_plan, then per layer muyo_cuda_paged_rope_append and
  * muyo_cuda_paged_attention_decode. Lengths, tables, slots and positions stay in device memory, so
  * the whole step can be captured in a CUDA graph and replayed; shapes and pointers are fixed at capture.
+ * Pointers are of the current device, which is the stream's. Outputs overlap no input, but where it says so.
  *
  * A pool (one for keys, one for values, of equal strides) holds num_pages pages of page_size slots.
  * Element (page, kv head, slot, channel) is at page * page_stride + head * head_stride +
@@ -566,7 +567,8 @@ int muyo_cuda_paged_attention_decode(const MuyoPagedAttentionParams* p, const fl
  * token keeps its relative accuracy. -inf logits (masked ids) have log p -inf; a row of nothing else
  * has log p -inf, entropy 0 and ids 0 .. top_k - 1. A row with a NaN or +inf gives NaN log
  * probabilities and entropy; NaN logits do not enter top_ids, and places that no id is left for hold -1.
- * logits are 4-byte aligned, in any stride. One call at a time may use a workspace. */
+ * logits are 4-byte aligned, in any stride; pointers are of the current device. One call at a time may use a
+ * workspace; it may hold anything before. */
 typedef struct MuyoTokenLogprobsParams {
     uint32_t rows, vocab;
     uint32_t stride; /* 0 = vocab */

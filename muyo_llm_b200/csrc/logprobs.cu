@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(kLogprobThreads, 4) k_logprob_pieces(LogprobDe
     const int token = __ldg(tokens + row);
     // float4 from the 16-byte border at or before the row's first logit; ids outside [begin, end) read as -inf
     const int origin = piece * p.tiles * TILE - (int)((reinterpret_cast<uintptr_t>(x) >> 2) & 3);
-    const int begin = max(origin, 0), end = min(origin + p.tiles * TILE, p.vocab);
+    const int begin = max(origin, 0), end = max(begin, min(origin + p.tiles * TILE, p.vocab));  // the last may be empty
     const int tiles = (end - origin + TILE - 1) / TILE;
     const auto quad = [&](int i) {
         if (i >= 0 && i <= p.vocab - 4)

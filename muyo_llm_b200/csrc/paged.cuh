@@ -1,6 +1,7 @@
 // Shared by the paged-cache entry points: the checked device view of MuyoPagedCache.
 #pragma once
 
+#include <atomic>
 #include <climits>
 #include <cmath>
 
@@ -54,6 +55,24 @@ inline int paged_prepare(const MuyoPagedCache& c, const char* what, PagedDev& d)
                  what);
     d.page_stride = (long long)ps, d.head_stride = (long long)hs, d.slot_stride = (long long)ss;
     return MUYO_OK;
+}
+
+// Lets `kernel` use `bytes` of dynamic shared memory on the current device. The setting stays with the function, so it
+// is made once per device (`done`: a bit each); the call costs the host as much as a fifth of a launch.
+template <typename Kernel>
+inline cudaError_t allow_smem(Kernel kernel, size_t bytes, std::atomic<unsigned long long>& done)
+{
+    int device = 0;
+    const cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess)
+        return e;
+    const unsigned long long bit = device < 64 ? 1ull << device : 0ull;
+    if (done.load(std::memory_order_acquire) & bit)
+        return cudaSuccess;
+    const cudaError_t r = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (r == cudaSuccess)
+        done.fetch_or(bit, std::memory_order_release);
+    return r;
 }
 
 // log2 of a power of two, or -1.

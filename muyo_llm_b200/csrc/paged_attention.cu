@@ -1058,7 +1058,8 @@ static int launch_paged_attention(const PagedAttnDev& d, const float* q, const v
 {
     using C = PagedTile<T, HD, WIDE>;
     auto kernel = k_paged_attention<T, HD, WIDE>;
-    MUYO_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM));
+    static std::atomic<unsigned long long> allowed{0};
+    MUYO_CUDA_TRY(allow_smem(kernel, C::SMEM, allowed));
     const int ctas = paged_attention_ctas(d, C::CTAS);
     PagedAttnDev e = d;
     e.one_page = d.c.page_size % C::KT == 0;

@@ -103,7 +103,7 @@ def test_strides_and_alignments(cuda, stride, vocab):
         check(logits, tokens, 11)
 
 
-@pytest.mark.parametrize("vocab", [40, 3001, 151936])
+@pytest.mark.parametrize("vocab", [40, 3001, 2046, 4094, 4095, 4096, 8190, 8192, 65534, 151936])
 def test_masks_and_ties(cuda, vocab):
     """Rows with -inf or the type's lowest value for all but a few, rows of one value, zeros of both signs, ties around
     the last alternative."""
@@ -138,6 +138,37 @@ def test_almost_certain_tokens(cuda, gap):
     if gap == 40.0:
         lp = score(logits, torch.tensor([17, 4999, 0], dtype=torch.int32, device="cuda"), 0)[0]
         assert bool((lp < 0).all())  # -4999 exp(-40) = -2e-14: not rounded to 0
+
+
+@pytest.mark.parametrize("rows", [1, 3, 30, 64, 200])
+def test_masked_tokens_of_many_rows(cuda, rows):
+    """Ranks of masked tokens and alternatives of masked rows, where rows are cut into pieces of every kind."""
+    vocab = 32766
+    g = gen(rows)
+    logits = torch.randn((rows, vocab), generator=g, device="cuda")
+    masked = torch.rand((rows, vocab), generator=g, device="cuda") < 0.999
+    logits[masked] = -math.inf
+    tokens = torch.randint(0, vocab, (rows,), generator=g, device="cuda").to(torch.int32)
+    check(logits[:12], tokens[:12], 32) if rows < 12 else None
+    lp, _, rk, ids, _ = score(logits, tokens, 32)
+    row, index = torch.arange(rows, device="cuda"), torch.arange(vocab, device="cuda")
+    given = logits[row, tokens.long()][:, None]
+    before = ((logits > given) | ((logits == given) & (index[None, :] < tokens[:, None]))).sum(1)
+    assert torch.equal(rk.long(), before)
+    assert torch.equal(ids.long(), torch.sort(logits, dim=1, descending=True, stable=True).indices[:, :32])
+    want = torch.log_softmax(logits.double(), 1)[row, tokens.long()]
+    same = (lp.double() == want) | ((lp.double() - want).abs() <= 400 * U)  # |d| below 12: (136 + 3 * 12) roundings
+    assert bool(same.all())
+
+
+def test_rising_rows(cuda):
+    """Every later logit larger, and by whole tiles: the list of what reaches the threshold runs over."""
+    vocab = 60000
+    rows = [torch.arange(vocab, device="cuda") * 1e-3, (torch.arange(vocab, device="cuda") // 4096).float(),
+            (torch.arange(vocab, device="cuda") % 1024).float() * 0.01]
+    logits = torch.stack(rows)
+    check(logits, torch.tensor([59999, 0, 1023], dtype=torch.int32, device="cuda"), 32)
+    check(logits.repeat(300, 1)[:4], torch.tensor([5, 59000, 7, 8], dtype=torch.int32, device="cuda"), 20)
 
 
 def test_nothing_left_nan_and_infinity(cuda):
