@@ -175,10 +175,10 @@ __device__ __forceinline__ void split_half2(float a, float b, uint32_t& hi, uint
     lo = pack_half2(a - h.x, b - h.y);
 }
 
-// x as two TF32: its leading 11 bits and the next 11.
+// x as two TF32: rounded to 11 bits, and 11 bits of what is left, of either sign: 23 bits without a bias.
 __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo)
 {
-    hi = __float_as_uint(x) & 0xffffe000u;
+    hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
     lo = __float_as_uint(x - __uint_as_float(hi)) & 0xffffe000u;
 }
 
