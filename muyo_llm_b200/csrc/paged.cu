@@ -16,7 +16,8 @@ namespace muyo {
 // finds its request by a binary search in the sums: all outputs are written in parallel from shared
 // memory, whatever the mix of long prompts and single tokens. A cluster of 8 CTAs shares that work; each forms
 // the sums for itself, and nothing is written before all have read what a step in place overwrites. Latency bound
-// (the sums, a binary search and a page look-up per token): one CTA took 69 us for 1501 requests with 48000 tokens.
+// (the sums, a binary search and a page look-up per token): 1501 requests with 48000 new tokens take 12 us, with one CTA
+// and divisions for pages and ring places 69 us; 250 single tokens 5 us, which is the call's own cost.
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanCtas = 8;
 constexpr int kPlanMaxSeqs = 8192;
@@ -70,7 +71,8 @@ __device__ __forceinline__ int page_of(const PlanDev& p, int slot)
     return p.page_shift >= 0 ? slot >> p.page_shift : slot / p.page_size;
 }
 
-__global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads) k_paged_plan(PlanDev p, const int32_t* cached_lens, const int32_t* new_lens,
+__global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads)
+                                                k_paged_plan(PlanDev p, const int32_t* cached_lens, const int32_t* new_lens,
                                                              int32_t* table, int32_t* ring, const int64_t* state,
                                                              int32_t* seq_lens, int32_t* query_start, int32_t* positions,
                                                              int32_t* slots, int64_t* state_out)
@@ -166,8 +168,8 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
     }
     // tokens
 #pragma unroll 2
-    for (int t = all; t < p.max_tokens; t += kPlanCtas * kPlanThreads) {
-        const int i = first_above(stop, p.seqs, t);
+    for (unsigned u = all; u < (unsigned)p.max_tokens; u += kPlanCtas * kPlanThreads) {  // the last step may pass 2^31
+        const int t = (int)u, i = first_above(stop, p.seqs, t);
         int slot = -1, pos = 0;
         if (i < p.seqs && (held[i] & kPlanAdmitted)) {
             const int c = (int)(held[i] & kPlanHeld);
@@ -183,14 +185,14 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
         positions[t] = pos;
     }
     // pages from the ring into the tables
-    for (int k = all; k < taken; k += kPlanCtas * kPlanThreads) {
-        const int i = first_above(upto, p.seqs, k);
+    for (unsigned u = all; u < (unsigned)taken; u += kPlanCtas * kPlanThreads) {
+        const int k = (int)u, i = first_above(upto, p.seqs, k);
         const int had = page_of(p, (int)(held[i] & kPlanHeld) + p.page_size - 1);
         table[(size_t)i * p.table_stride + had + k - (i > 0 ? upto[i - 1] : 0)] = ring[ring_index(first, k, p.num_pages)];
     }
     // pages of ended requests into the ring
-    for (int k = all; k < back; k += kPlanCtas * kPlanThreads) {
-        const int i = first_above(gone, p.seqs, k);
+    for (unsigned u = all; u < (unsigned)back; u += kPlanCtas * kPlanThreads) {
+        const int k = (int)u, i = first_above(gone, p.seqs, k);
         ring[ring_index(last, k, p.num_pages)] = table[(size_t)i * p.table_stride + k - (i > 0 ? gone[i - 1] : 0)];
     }
     if (all == 0) {
@@ -289,7 +291,10 @@ __device__ __forceinline__ void turn(float& a, float& b, double c, double s)
 // One CTA per token. The angles are formed once per token, in float64 as k_kv_append forms them, and shared by its
 // heads. V4: a thread's unit is two float4 of a row - four pairs, or eight channels that pass unchanged, or eight
 // channels of v - all loaded before the angles are waited for; else a unit is one pair. Bound by the bytes
-// (q twice, k and v once, the pools' rows); float64 costs 10 operations a pair, far below the memory time.
+// (q twice, k and v once, the pools' rows): 6001 tokens of 32/8 heads of 128 into an e4m3 pool, 259 MB, take 55 us (4.7
+// TB/s, 0.72 of the copy rate); the float64 rotation costs 1.5 us of it. A CTA that takes several tokens with the next
+// one's loads under way was slower (63 us in registers, 97 us through shared memory): CTAs of one token are dealt out as
+// SMs come free.
 constexpr int kAppendThreads = 256;
 
 template <typename KV, bool V4>
@@ -405,7 +410,8 @@ __global__ void __launch_bounds__(kAppendThreads, 4) k_paged_append(AppendDev p,
                 j0 = j0 < p.n_offs ? j0 : j0 + p.n_dims;
                 j1 = j0 + 1;
             }
-            const float* x = h < heads ? q + t * p.stride_q + (long long)h * hd : k + t * p.stride_k + (long long)(h - heads) * hd;
+            const float* x = h < heads ? q + t * p.stride_q + (long long)h * hd
+                                       : k + t * p.stride_k + (long long)(h - heads) * hd;
             float y0 = x[j0], y1 = x[j1];
             if (i < half)
                 turn(y0, y1, cs[i], cs[half + i]);

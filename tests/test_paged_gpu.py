@@ -161,6 +161,24 @@ def test_plan_without_tokens_buffer(cuda):
     assert list(run_plan(*args, 4, 0)) == list(plan_reference(*args, 4, 0))
 
 
+def test_plan_with_the_largest_max_tokens(cuda):
+    """Every place of buffers of 2^31 - 2 tokens is written, and none behind them."""
+    tokens = (1 << 31) - 2
+    if torch.cuda.mem_get_info()[0] < 20 << 30:
+        pytest.skip("needs 20 GB")
+    p = nodes.paged_plan_params(2, page_size=16, num_pages=8, table_stride=4, max_tokens=tokens)
+    positions, slots = (torch.full((tokens + 2,), 77, dtype=torch.int32, device="cuda") for _ in range(2))
+    table = torch.full((2, 4), -1, dtype=torch.int32, device="cuda")
+    lens, starts, state = ints([0, 0]), ints([0, 0, 0]), torch.tensor([0, 8, 0, 0], device="cuda")
+    nodes.paged_plan(p, ints([0, 0]), ints([3, 20]), table, torch.arange(8, dtype=torch.int32, device="cuda"), state, lens, starts,
+                     positions, slots, state)
+    torch.cuda.synchronize()
+    assert slots[:23].tolist() == [*range(3), *range(16, 36)] and positions[:23].tolist() == [*range(3), *range(20)]
+    assert bool((slots[23:tokens] == -1).all()) and bool((positions[23:tokens] == 0).all())
+    assert slots[tokens:].tolist() == positions[tokens:].tolist() == [77, 77]
+    assert lens.tolist() == [3, 20] and state.tolist() == [3, 8, 0, 23]
+
+
 @pytest.mark.parametrize("state", [(10, 5), (0, 1 << 40), (-7, 3)])
 def test_plan_survives_bad_content(cuda, state):
     """Lengths past the row, page numbers and counters that make no sense: nothing is touched out of bounds, lengths and
@@ -543,6 +561,20 @@ def test_attention_agrees_with_contiguous(cuda):
     torch.cuda.synchronize()
     _, _, tol, _ = attention64(q.double().reshape(heads, hd), K[:, :n].transpose(0, 1).double(), V[:, :n].transpose(0, 1).double(), 0.125)
     assert bool(((out[0] - want).abs().double() <= 2 * tol.reshape(-1)).all())
+
+
+@pytest.mark.parametrize("window", [0, 50])
+def test_attention_of_prompt_tokens(cuda, window):
+    """Each token of a prompt as a row: its request's table row again, the keys up to its own."""
+    heads, kv, hd, page = 14, 2, 64, 16
+    prompts = [70, 1, 33]
+    g = gen(14)
+    cache, pools, table, values, rows = make_paged(prompts, kv, hd, _abi.KV_F16, "nhd", page, g)
+    owner = [i for i, n in enumerate(prompts) for _ in range(n)]
+    lens = [t + 1 for n in prompts for t in range(n)]
+    q = randn((len(lens), heads * hd), g, 2.0)
+    out, lse = run_attention(cache, heads, kv, hd, q, pools, table[owner].contiguous(), lens, window=window)
+    check_attention(out, lse, q, values, [rows[i][:n] for i, n in zip(owner, lens)], lens, heads, kv, hd, window, 0.125)
 
 
 def test_attention_repeats_bit_for_bit(cuda):
