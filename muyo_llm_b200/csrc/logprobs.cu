@@ -88,7 +88,7 @@ __device__ __forceinline__ int logprob_equal_ids(const float* x, float value, in
     int id = -1;
 #pragma unroll 1
     for (int i = begin; have < top_k && i < end; i += 32) {
-        const unsigned equal = __ballot_sync(0xffffffffu, i + lane < end && __ldg(x + min(i + lane, end - 1)) == value);
+        const unsigned equal = __ballot_sync(0xffffffffu, i + lane < end && x[min(i + lane, end - 1)] == value);
         if (lane >= have && lane < top_k && lane - have < __popc(equal)) {
             unsigned bits = equal;
 #pragma unroll 1
@@ -173,11 +173,16 @@ __device__ __forceinline__ LogprobPiece logprob_join_sums(const LogprobDev& p, L
 // are ordered by counting. -inf is never listed, its places are filled in at the end. Masses at the threshold (a
 // constant row, a mask of the lowest value) run the list over: then what lies above it is listed, and of the equal
 // ones the lowest ids.
+//
+// Bound by the read, 4 bytes a logit: 2001 rows of 32001, 256 MB, take 56 us (4.6 TB/s, 0.70 of the copy rate; a CTA's
+// first loads and its last sums are a third of its time), 97 rows of 151936 with 20 alternatives, 59 MB, 23.5 us (the
+// loop ends at 40% of the kernel's time, the rest is the second reads and the cluster's join), one row 8.5 us. Listing
+// tile by tile in the loop took 40 us for the 97 rows, whole pieces in shared memory 59 us.
 template <bool TOP, int V>
-__global__ void __launch_bounds__(kLogprobThreads, 4) k_logprob_pieces(LogprobDev p, const float* __restrict__ logits,
-                                                                       const int32_t* __restrict__ tokens,
-                                                                       LogprobPiece* __restrict__ stats,
-                                                                       unsigned long long* __restrict__ tops, LogprobOut out)
+__global__ void __launch_bounds__(kLogprobThreads, 4) k_logprob_pieces(LogprobDev p, const float* logits,
+                                                                       const int32_t* tokens,
+                                                                       LogprobPiece* stats,
+                                                                       unsigned long long* tops, LogprobOut out)
 {
     constexpr int WARPS = kLogprobWarps, Q = kLogprobThreads * 4, TILE = V * Q;
     __shared__ float s_m[WARPS], s_r[WARPS], s_e[WARPS], s_mine[TOP ? kLogprobThreads : 1], s_threshold;
@@ -189,7 +194,7 @@ __global__ void __launch_bounds__(kLogprobThreads, 4) k_logprob_pieces(LogprobDe
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int row = blockIdx.x / p.pieces, piece = blockIdx.x - row * p.pieces;
     const float* x = logits + row * p.stride;
-    const int token = __ldg(tokens + row);
+    const int token = tokens[row];
     // float4 from the 16-byte border at or before the row's first logit; ids outside [begin, end) read as -inf
     const int origin = piece * p.tiles * TILE - (int)((reinterpret_cast<uintptr_t>(x) >> 2) & 3);
     const int begin = max(origin, 0), end = max(begin, min(origin + p.tiles * TILE, p.vocab));  // the last may be empty
@@ -200,7 +205,7 @@ __global__ void __launch_bounds__(kLogprobThreads, 4) k_logprob_pieces(LogprobDe
         float4 f = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
-            const float y = i + c >= 0 && i + c < p.vocab ? __ldg(x + i + c) : -INFINITY;
+            const float y = i + c >= 0 && i + c < p.vocab ? x[i + c] : -INFINITY;
             f.x = c == 0 ? y : f.x, f.y = c == 1 ? y : f.y, f.z = c == 2 ? y : f.z, f.w = c == 3 ? y : f.w;
         }
         return f;
@@ -223,7 +228,7 @@ __global__ void __launch_bounds__(kLogprobThreads, 4) k_logprob_pieces(LogprobDe
     };
     float4 va[V], vb[V];
     load(va, 0);
-    const float xt = token >= 0 && token < p.vocab ? __ldg(x + token) : INFINITY;  // outside: nothing in front
+    const float xt = token >= 0 && token < p.vocab ? x[token] : INFINITY;  // outside: nothing in front
     // An id below the token is in front of it at an equal logit too: it is compared with the next value below. Below -inf
     // there is none: of a masked token, all ids below it are in front (added after the loop) and those above it that are
     // not masked. The four logits around the token have both kinds: put right after the loop.
@@ -277,7 +282,7 @@ __global__ void __launch_bounds__(kLogprobThreads, 4) k_logprob_pieces(LogprobDe
         if (token >= begin && token < end) {
 #pragma unroll 1
             for (int i = max(token - ((token - origin) & 3), 0); i < token; ++i)
-                before += xt == -INFINITY ? -(__ldg(x + i) > xt) : __ldg(x + i) == xt;
+                before += xt == -INFINITY ? -(x[i] > xt) : x[i] == xt;
         }
         if (xt == -INFINITY)
             before += min(max(token - begin, 0), end - begin);
@@ -454,7 +459,7 @@ __global__ void __launch_bounds__(kLogprobThreads, 4) k_logprob_pieces(LogprobDe
                 unsigned long long next = 0ull;
 #pragma unroll 4
                 for (int i = begin + tid; i < end; i += kLogprobThreads) {
-                    const float y = __ldg(x + i);
+                    const float y = x[i];
                     const unsigned long long key = y > -INFINITY ? order_key(y, i) : 0ull;
                     next = key < last && key > next ? key : next;
                 }
@@ -489,7 +494,8 @@ __global__ void __launch_bounds__(kLogprobThreads, 4) k_logprob_pieces(LogprobDe
             if (TOP && tid < p.pieces * p.top_k)  // at most 256 keys
                 s_list[tid] = cluster.map_shared_rank(s_top, tid / p.top_k)[tid % p.top_k];
             if (warp == 0)
-                sum = logprob_join_sums(p, *cluster.map_shared_rank(&s_sum, min((unsigned)lane, (unsigned)p.pieces - 1)), p.pieces);
+                sum = logprob_join_sums(
+                    p, *cluster.map_shared_rank(&s_sum, min((unsigned)lane, (unsigned)p.pieces - 1)), p.pieces);
         }
         cluster.sync();  // the others' shared memory is read
         if (piece > 0)
@@ -507,10 +513,10 @@ __global__ void __launch_bounds__(kLogprobThreads, 4) k_logprob_pieces(LogprobDe
 }
 
 // Joins a row's pieces where they are more than a cluster: one CTA per row, a piece per thread at a time.
-__global__ void __launch_bounds__(kLogprobJoinThreads) k_logprob_join(LogprobDev p, const float* __restrict__ logits,
-                                                                      const int32_t* __restrict__ tokens,
-                                                                      const LogprobPiece* __restrict__ stats,
-                                                                      const unsigned long long* __restrict__ tops,
+__global__ void __launch_bounds__(kLogprobJoinThreads) k_logprob_join(LogprobDev p, const float* logits,
+                                                                      const int32_t* tokens,
+                                                                      const LogprobPiece* stats,
+                                                                      const unsigned long long* tops,
                                                                       LogprobOut out)
 {
     constexpr int WARPS = kLogprobJoinThreads / 32;
@@ -522,7 +528,7 @@ __global__ void __launch_bounds__(kLogprobJoinThreads) k_logprob_join(LogprobDev
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = blockIdx.x;
     const LogprobPiece* mine = stats + (size_t)row * p.pieces;
     const int token = tokens[row];
-    const float xt = token >= 0 && token < p.vocab ? __ldg(logits + row * p.stride + token) : 0.0f;
+    const float xt = token >= 0 && token < p.vocab ? logits[row * p.stride + token] : 0.0f;
     float m = -INFINITY;
 #pragma unroll 1
     for (int c = tid; c < p.pieces; c += kLogprobJoinThreads)
@@ -618,7 +624,8 @@ static int logprobs_prepare(const MuyoTokenLogprobsParams* p, LogprobDev& d)
     // A row is cut into the pieces that come nearest to three CTAs on an SM (97 rows of 151936 with 20 alternatives: 5
     // pieces 23.5 us, 6 pieces 30 us, the ends of more pieces cost more than their loops gain; 150 rows: 2 pieces 44
     // us, 3 pieces 34 us), and not into more than a cluster joins where those are a CTA per SM (40 rows: 8 pieces 20
-    // us, 14 pieces and a second kernel 22 us; one row: 8 pieces 13 us, 75 pieces 8 us). A row may begin 3 logits behind a 16-byte border.
+    // us, 14 pieces and a second kernel 22 us; one row: 8 pieces 13 us, 75 pieces 8 us). A row may begin 3 logits
+    // behind a 16-byte border.
     const long long large = (d.vocab + 3LL + 16 * kLogprobThreads - 1) / (16 * kLogprobThreads);
     d.small = large * d.rows < sm_count();  // the larger tiles would leave SMs without a CTA
     const long long tiles = d.small ? (d.vocab + 3LL + 8 * kLogprobThreads - 1) / (8 * kLogprobThreads) : large;

@@ -5,17 +5,24 @@
 // the cache's bytes: 2 * keys * kv_heads * head_dim * sizeof(element).
 //
 // Work. The keys of a (request, KV head) are cut into tiles of KT keys (8 KB of keys and values, fewer for
-// small heads); all tiles of the batch, in order, are dealt out evenly and contiguously to the warps of one
-// CTA per SM. The dealing is done on the device from seq_lens (a scan per CTA), so a captured graph stays
-// right when lengths change, and no length spread leaves SMs idle: one request over 131071 keys and 200
-// requests over 60 to 2048 keys both keep every warp busy to within one tile. A warp that holds the whole of a
-// segment (the tiles of one request and KV head) writes its output; pieces of segments cut by a warp's border
-// are joined in shared memory by the CTA, those cut by a CTA's border by a second kernel from at most two
+// small heads); all tiles of the batch, in order, are dealt out evenly and contiguously to the warps of CTAs of
+// four warps, as many as are on the SMs at once. The dealing is done on the device from seq_lens (a scan per CTA), so a
+// captured graph stays right when lengths change, and no spread of lengths leaves warps idle: one request over
+// 131071 keys and 200 requests over 60 to 2048 keys both keep every warp busy to within one tile. A warp that holds the
+// whole of a segment (the tiles of one request and KV head) writes its output; pieces of segments cut by a warp's
+// border are joined in shared memory by the CTA, those cut by a CTA's border by a second kernel from at most two
 // partials per CTA (m, l, o).
 //
 // A warp copies its tiles with cp.async into a ring of its own (no block barriers) STAGES - 1 tiles ahead;
 // the page numbers are fetched one tile further ahead. Rows are swizzled by 16-byte chunks so that the
 // fragment reads below meet no bank conflicts at 128-byte rows and wider.
+//
+// Measured: 131071 keys of 32/8 heads of 128 in F16, 537 MB, 99 us (5.4 TB/s, 0.83 of the copy rate; the SMs of some
+// GPCs stream 12% slower than the others, and even shares wait for them); 64 requests over 2000 to 16000 e4m3 keys,
+// 901 MB, 187 us (4.8 TB/s, 0.74; the conversions' dependent chains with 8 warps on an SM - twice the warps with tiles of
+// half the size: 214 us); 200 requests over 60 to 2048 keys of 14/2 heads of 64 in F16, 60 MB, 23 us (start, joins and
+// the second kernel are two thirds); one request over 1023 keys 8.4 us (two launches); 33 requests of 16 heads on one
+// F32 head, windows of 4096 keys, 80 MB, 42 us (the splitting of F32 operands).
 //
 // Products. mma.sync tiles of 16 rows x 8 keys (scores) and 16 rows x 8 channels (values). With at most 8 query
 // heads per KV head the 16 rows are the heads' leading halves and, below them, their remainders: an F32
@@ -58,8 +65,10 @@ struct PagedTile {
     static constexpr int RB = HD * ES;        // bytes of a row
     static constexpr int CPR = RB / 16;       // 16-byte chunks of a row
     static constexpr int KSTEP = T == MUYO_KV_F32 ? 8 : 16;
+    // 4 KB of keys: half of that with three CTAs on an SM took 214 us where this takes 190 (64 requests, e4m3). At most
+    // 64: a warp votes and masks two keys a lane.
     static constexpr int KT = kPagedTile / RB > 64 ? 64 : kPagedTile / RB < KSTEP ? KSTEP : kPagedTile / RB;  // keys of a tile
-    static constexpr int STAGES = WIDE ? 2 : 3;
+    static constexpr int STAGES = WIDE ? 2 : 3;  // WIDE: a third would leave shared memory for one CTA
     static constexpr int TILE = KT * RB;      // bytes of a tile's keys (or values)
     static constexpr int ROWS = WIDE ? 16 : 8;
     static constexpr int PART = ROWS * (HD + 2);  // floats of a partial: o [ROWS][HD], m, l
@@ -76,7 +85,9 @@ struct PagedTile {
     static_assert(KT % KSTEP == 0 && KT * CPR % 32 == 0, "tile shape");
     static_assert(RING >= PART * 4, "a drained ring holds a partial");
     static constexpr size_t SMEM = (size_t)kPagedWarps * (RING + PART * 4);
-    static constexpr int CTAS = SMEM <= 75 * 1024 ? 3 : 2;  // on an SM at once
+    // On an SM at once. Three where they fit; two of full tiles: twice the CTAs, half of them waiting for their turn,
+    // took 108 us where one turn takes 99 (131071 keys) and 29 us where it takes 23 (200 requests).
+    static constexpr int CTAS = SMEM <= 75 * 1024 ? 3 : 2;
 };
 
 template <int CPR>
@@ -239,7 +250,7 @@ struct PagedCursor {
             h = 0;
 #pragma unroll 1
             do {
-                span = PagedSpan<KT>(p, __ldg(lens + ++s));
+                span = PagedSpan<KT>(p, lens[++s]);
             } while (span.t1 == span.t0);
         }
         t = span.t0;
@@ -268,9 +279,8 @@ struct PagedGroup {
 
 template <int T, int HD, bool WIDE>
 __global__ void __launch_bounds__(kPagedThreads, (PagedTile<T, HD, WIDE>::CTAS))
-k_paged_attention(PagedAttnDev p, const float* __restrict__ q, const char* __restrict__ k_pool,
-                  const char* __restrict__ v_pool, const int32_t* __restrict__ table, const int32_t* __restrict__ lens,
-                  float* __restrict__ out, float* __restrict__ lse, float* __restrict__ part, PagedDesc* __restrict__ descs)
+k_paged_attention(PagedAttnDev p, const float* q, const char* k_pool, const char* v_pool, const int32_t* table,
+                  const int32_t* lens, float* out, float* lse, float* part, PagedDesc* descs)
 {
     using C = PagedTile<T, HD, WIDE>;
     constexpr int KT = C::KT, HR = WIDE ? 2 : 1;  // HR: heads of a lane
@@ -303,7 +313,7 @@ k_paged_attention(PagedAttnDev p, const float* __restrict__ q, const char* __res
     int mine = 0, empty = 0;
 #pragma unroll 1
     for (int s = s_begin; s < s_end; ++s) {
-        const PagedSpan<KT> span(p, __ldg(lens + s));
+        const PagedSpan<KT> span(p, lens[s]);
         mine += (span.t1 - span.t0) * p.c.kv_heads;
         empty |= span.t1 == span.t0;
     }
@@ -337,7 +347,7 @@ k_paged_attention(PagedAttnDev p, const float* __restrict__ q, const char* __res
     if (empty) {  // requests without keys
 #pragma unroll 1
         for (int s = blockIdx.x * W + warp; s < p.seqs; s += gridDim.x * W) {
-            const PagedSpan<KT> span(p, __ldg(lens + s));
+            const PagedSpan<KT> span(p, lens[s]);
             if (span.t1 > span.t0)
                 continue;
 #pragma unroll 1
@@ -367,7 +377,7 @@ k_paged_attention(PagedAttnDev p, const float* __restrict__ q, const char* __res
         cur.s = share * per;
 #pragma unroll 1
         for (;; ++cur.s) {
-            cur.span = PagedSpan<KT>(p, __ldg(lens + cur.s));
+            cur.span = PagedSpan<KT>(p, lens[cur.s]);
             tiles = cur.span.t1 - cur.span.t0;
             if (rest < tiles * p.c.kv_heads)
                 break;
@@ -396,14 +406,14 @@ k_paged_attention(PagedAttnDev p, const float* __restrict__ q, const char* __res
             const int at = p.page_shift >= 0 ? key >> p.page_shift : key / p.c.page_size;
             pages[i] = -1;
             if (p.one_page ? i == 0 : (KT % 32 == 0 || lane < KT) && key < load.span.n && key >= load.span.begin)
-                pages[i] = __ldg(table + (size_t)load.s * p.table_stride + at);
+                pages[i] = table[(size_t)load.s * p.table_stride + at];
         }
         if (begins) {  // the segment's q into L1: behind the copies it would wait for them
             const float* qrow = q + load.s * p.stride_q + (long long)load.h * p.c.group * HD;
 #pragma unroll 1
             for (int d = lane * 32; d < p.c.group * HD; d += 32 * 32) {
                 float unused;
-                asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(unused) : "l"(qrow + d));
+                asm volatile("ld.global.f32 %0, [%1];" : "=f"(unused) : "l"(qrow + d));
             }
         }
     };
@@ -433,13 +443,13 @@ k_paged_attention(PagedAttnDev p, const float* __restrict__ q, const char* __res
                 }
             } else {
 #pragma unroll 1
-            for (int i = 0; i < KT * C::CPR / 32; ++i) {
-                const int row = i * RPI + row0;
-                const bool seen = row >= lo && row < hi;
-                copy16(kd + row * C::RB + k_chunk<C::CPR>(row, ch) * 16, seen ? kp : k_pool, seen);
-                copy16(vd + row * C::RB + v_chunk<C::CPR>(row, ch) * 16, seen ? vp : v_pool, seen);
-                kp += RPI * slot_bytes, vp += RPI * slot_bytes;
-            }
+                for (int i = 0; i < KT * C::CPR / 32; ++i) {
+                    const int row = i * RPI + row0;
+                    const bool seen = row >= lo && row < hi;
+                    copy16(kd + row * C::RB + k_chunk<C::CPR>(row, ch) * 16, seen ? kp : k_pool, seen);
+                    copy16(vd + row * C::RB + v_chunk<C::CPR>(row, ch) * 16, seen ? vp : v_pool, seen);
+                    kp += RPI * slot_bytes, vp += RPI * slot_bytes;
+                }
             }
         } else {
             long long off[(KT + 31) / 32];
@@ -484,7 +494,7 @@ k_paged_attention(PagedAttnDev p, const float* __restrict__ q, const char* __res
                 const int d = (4 * (k / SPC) + cq) * C::EPC + (k % SPC) * C::KPS;
 #pragma unroll
                 for (int e = 0; e < C::KPS; e += 2) {
-                    const float2 x = head < p.c.group ? __ldg(reinterpret_cast<const float2*>(qrow + head * HD + d + e))
+                    const float2 x = head < p.c.group ? *reinterpret_cast<const float2*>(qrow + head * HD + d + e)
                                                       : make_float2(0.0f, 0.0f);
                     raw[r][k * C::KPS + e] = x.x;
                     raw[r][k * C::KPS + e + 1] = x.y;
@@ -948,9 +958,8 @@ constexpr int kJoinThreads = 512;
 constexpr int kJoinPieces = 480;  // one per CTA at most
 
 template <int HD, int ROWS>
-__global__ void __launch_bounds__(kJoinThreads) k_paged_join(PagedAttnDev p, const float* __restrict__ part,
-                                                             const PagedDesc* __restrict__ descs, float* __restrict__ out,
-                                                             float* __restrict__ lse)
+__global__ void __launch_bounds__(kJoinThreads) k_paged_join(PagedAttnDev p, const float* part, const PagedDesc* descs,
+                                                             float* out, float* lse)
 {
     constexpr int PART = ROWS * (HD + 2), Q = HD / 4;
     __shared__ float s_w[ROWS][kJoinPieces];
@@ -1017,7 +1026,7 @@ static int paged_attention_prepare(const MuyoPagedAttentionParams* p, PagedAttnD
     const int rc = paged_prepare(p->cache, "paged_attention", d.c);
     if (rc != MUYO_OK)
         return rc;
-    MUYO_REQUIRE(p->seqs > 0 && p->seqs <= (uint32_t)INT_MAX, "paged_attention: seqs must be in [1, INT32_MAX]");
+    MUYO_REQUIRE(p->seqs > 0 && p->seqs <= 1u << 28, "paged_attention: seqs must be in [1, 2^28]");
     MUYO_REQUIRE(p->table_stride > 0 && (uint64_t)p->cache.page_size * p->table_stride <= (uint64_t)1 << 30,
                  "paged_attention: table_stride %u must be positive, and a row at most 2^30 slots", p->table_stride);
     MUYO_REQUIRE(p->window <= (uint32_t)INT_MAX, "paged_attention: window %u exceeds INT32_MAX", p->window);
@@ -1122,10 +1131,13 @@ extern "C" int muyo_cuda_paged_attention_decode(const MuyoPagedAttentionParams* 
     MUYO_REQUIRE(aligned16(workspace), "paged_attention: workspace must be 16-byte aligned");
     switch (p->cache.kv_dtype) {
         case MUYO_KV_F32:
-            return launch_paged_attention_dim<MUYO_KV_F32>(d, q, k_pool, v_pool, block_table, seq_lens, out, lse, workspace, stream);
+            return launch_paged_attention_dim<MUYO_KV_F32>(d, q, k_pool, v_pool, block_table, seq_lens, out, lse, workspace,
+                                                           stream);
         case MUYO_KV_F16:
-            return launch_paged_attention_dim<MUYO_KV_F16>(d, q, k_pool, v_pool, block_table, seq_lens, out, lse, workspace, stream);
+            return launch_paged_attention_dim<MUYO_KV_F16>(d, q, k_pool, v_pool, block_table, seq_lens, out, lse, workspace,
+                                                           stream);
         default:
-            return launch_paged_attention_dim<MUYO_KV_F8>(d, q, k_pool, v_pool, block_table, seq_lens, out, lse, workspace, stream);
+            return launch_paged_attention_dim<MUYO_KV_F8>(d, q, k_pool, v_pool, block_table, seq_lens, out, lse, workspace,
+                                                           stream);
     }
 }

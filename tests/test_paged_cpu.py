@@ -66,7 +66,7 @@ def attention(**kw):
 
 
 @pytest.mark.parametrize("kw,match", [
-    (dict(seqs=0), "seqs"), (dict(seqs=1 << 31), "seqs"), (dict(table_stride=0), "table_stride"),
+    (dict(seqs=0), "seqs"), (dict(seqs=1 << 31), "seqs"), (dict(seqs=(1 << 28) + 1), "seqs"), (dict(table_stride=0), "table_stride"),
     (dict(table_stride=1 << 28), "2^30"), (dict(window=1 << 31), "window"), (dict(scale=float("nan")), "scale"),
     (dict(stride_q=892), "row stride"), (dict(stride_out=892), "row stride"), (dict(stride_q=898), "multiples of 4"),
 ])
