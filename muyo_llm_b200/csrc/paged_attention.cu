@@ -193,12 +193,12 @@ __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo)
     lo = __float_as_uint(x - __uint_as_float(hi)) & 0xffffe000u;
 }
 
-// Two e4m3 (the low 16 bits) as two F16, exactly.
-__device__ __forceinline__ uint32_t e4m3x2_half2(uint32_t v)
+// Four e4m3 as F16 pairs, exactly: the two low bytes, the two high ones.
+__device__ __forceinline__ void e4m3x4_half2(uint32_t v, uint32_t& low, uint32_t& high)
 {
-    uint32_t r;
-    asm("{.reg .b16 t; cvt.u16.u32 t, %1; cvt.rn.f16x2.e4m3x2 %0, t;}" : "=r"(r) : "r"(v));
-    return r;
+    asm("{.reg .b16 x, y; mov.b32 {x, y}, %2; cvt.rn.f16x2.e4m3x2 %0, x; cvt.rn.f16x2.e4m3x2 %1, y;}"
+        : "=r"(low), "=r"(high)
+        : "r"(v));
 }
 
 template <int BYTES>
@@ -600,7 +600,7 @@ k_paged_attention(PagedAttnDev p, const float* q, const char* k_pool, const char
                         if constexpr (T == MUYO_KV_F16) {
                             b0 = ch.w[2 * j2], b1 = ch.w[2 * j2 + 1];
                         } else {
-                            b0 = e4m3x2_half2(ch.w[j2]), b1 = e4m3x2_half2(ch.w[j2] >> 16);
+                            e4m3x4_half2(ch.w[j2], b0, b1);
                         }
                         if constexpr (WIDE) {
                             const uint32_t lo[4] = {qf[k * 8 + 4], qf[k * 8 + 5], qf[k * 8 + 6], qf[k * 8 + 7]};
@@ -744,32 +744,39 @@ k_paged_attention(PagedAttnDev p, const float* q, const char* k_pool, const char
                         v[j][e].load(vs + row * C::RB + v_chunk<C::CPR>(row, byte >> 4) * 16 + (byte & 15));
                     }
 #pragma unroll
-                for (int n = 0; n < C::VE; ++n) {
-                    float acc[4];
+                for (int n = 0; n < C::VE; n += 2) {  // two channels of both keys of a pair from one word of each
+                    float acc[2][4];
 #pragma unroll
                     for (int j = 0; j < KT / 16; ++j) {
-                        uint32_t b[2];
+                        uint32_t b[2][2];
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
                             if constexpr (T == MUYO_KV_F16) {
-                                b[h] = __byte_perm(v[j][2 * h].w[n >> 1], v[j][2 * h + 1].w[n >> 1], n & 1 ? 0x7632 : 0x5410);
-                            } else {  // bytes n of both keys
-                                b[h] = e4m3x2_half2(__byte_perm(v[j][2 * h].w[n >> 2], v[j][2 * h + 1].w[n >> 2],
-                                                                (n & 3) | ((n & 3) + 4) << 4));
+                                const uint32_t x = v[j][2 * h].w[n >> 1], y = v[j][2 * h + 1].w[n >> 1];
+                                b[0][h] = __byte_perm(x, y, 0x5410), b[1][h] = __byte_perm(x, y, 0x7632);
+                            } else {
+                                const uint32_t x = v[j][2 * h].w[n >> 2], y = v[j][2 * h + 1].w[n >> 2];
+                                e4m3x4_half2(__byte_perm(x, y, n & 2 ? 0x7362 : 0x5140), b[0][h], b[1][h]);
                             }
                         }
-                        if constexpr (WIDE) {
-                            const uint32_t lo[4] = {w[j][4], w[j][5], w[j][6], w[j][7]};
-                            const uint32_t hi[4] = {w[j][0], w[j][1], w[j][2], w[j][3]};
-                            j == 0 ? mma_f16_first(acc, lo, b[0], b[1]) : mma_f16(acc, lo, b[0], b[1]);
-                            mma_f16(acc, hi, b[0], b[1]);
-                        } else {
-                            const uint32_t a[4] = {w[j][0], w[j][1], w[j][2], w[j][3]};
-                            j == 0 ? mma_f16_first(acc, a, b[0], b[1]) : mma_f16(acc, a, b[0], b[1]);
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            if constexpr (WIDE) {
+                                const uint32_t lo[4] = {w[j][4], w[j][5], w[j][6], w[j][7]};
+                                const uint32_t hi[4] = {w[j][0], w[j][1], w[j][2], w[j][3]};
+                                j == 0 ? mma_f16_first(acc[e], lo, b[e][0], b[e][1]) : mma_f16(acc[e], lo, b[e][0], b[e][1]);
+                                mma_f16(acc[e], hi, b[e][0], b[e][1]);
+                            } else {
+                                const uint32_t a[4] = {w[j][0], w[j][1], w[j][2], w[j][3]};
+                                j == 0 ? mma_f16_first(acc[e], a, b[e][0], b[e][1]) : mma_f16(acc[e], a, b[e][0], b[e][1]);
+                            }
                         }
                     }
-                    float(&on)[2 * HR] = o[ic * C::VE + n];
-                    add_tile(on, alpha, acc);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float(&on)[2 * HR] = o[ic * C::VE + n + e];
+                        add_tile(on, alpha, acc[e]);
+                    }
                 }
             }
         }
