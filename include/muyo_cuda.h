@@ -468,7 +468,8 @@ int muyo_p2p_destroy(MuyoP2PGroup* g);
  * slot * slot_stride + channel. Strides of 0 mean the packed order [page][kv_head][slot][channel]
  * (all three or none are 0). Pools are 16-byte aligned and strides are multiples of 16 bytes. A slot's
  * number is page * page_size + slot. An element of an F8 (e4m3) pool, or of any pool, stands for
- * its value times k_scale or v_scale (0 is read as 1); what does not fit e4m3 is stored as +-448. */
+ * its value times k_scale or v_scale (in [2^-100, 2^100]; 0 is read as 1); what does not fit e4m3 is
+ * stored as +-448. */
 #define MUYO_KV_F8 2u /* e4m3, paged pools only */
 typedef struct MuyoPagedCache {
     uint32_t heads, kv_heads, head_dim; /* head_dim 16, 32, 64 or 128; at most 16 query heads per KV head */
@@ -519,7 +520,8 @@ int muyo_cuda_rope_frequencies(const MuyoRopeParams* p, const float* freq_factor
  * angles, rotation in float64 rounded once, as muyo_cuda_kv_append): NEOX pairs channels
  * (j, j + n_dims/2), NORMAL pairs (2j, 2j + 1), of the n_dims channels from n_offs; the others pass
  * unchanged. The turned q goes to q_out (which may be q with the same stride), the turned k and the
- * v, divided by their scales and rounded to the pool's type, to slot slots[t] of their pools. A token
+ * v, divided by their scales (F16 and F8: times the scale's F32 reciprocal) and rounded to the pool's
+ * type, to slot slots[t] of their pools. A token
  * with a slot outside [0, num_pages * page_size) is left out: no q_out row, no pool is written.
  * Slots of one call must differ from one another: of two tokens in one slot either may stay, channel
  * by channel. q may be NULL (keys and values only). n_dims 0 turns nothing and reads no freqs. */

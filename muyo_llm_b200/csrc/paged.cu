@@ -226,12 +226,6 @@ __global__ void k_rope_frequencies(int pairs, double base, double freq_scale, do
 }
 
 // ---- rotary positions + append -----------------------------------------------------------------------
-struct AppendDev {
-    PagedDev c;
-    int mode, n_dims, n_offs;
-    long long stride_q, stride_k, stride_v, stride_q_out;
-    int has_q;
-};
 
 template <typename KV>
 __device__ __forceinline__ KV pool_round(float v);
@@ -274,11 +268,32 @@ __device__ __forceinline__ void pool_store4<__nv_fp8_e4m3>(__nv_fp8_e4m3* dst, f
     *reinterpret_cast<unsigned*>(dst) = a | b << 16;
 }
 
-__device__ __forceinline__ float4 scaled_down(float4 v, float scale)
-{
-    return scale == 1.0f ? v : make_float4(__fdiv_rn(v.x, scale), __fdiv_rn(v.y, scale), __fdiv_rn(v.z, scale),
-                                           __fdiv_rn(v.w, scale));
-}
+// x / scale for the pool. To F16 and e4m3, whose rounding is 2^13 times and more as coarse, as a product with the
+// scale's reciprocal, which is two roundings of F32 (6001 tokens into an e4m3 pool: 46.7 us, by division 49.2 us).
+struct PoolScale {
+    float scale, inverse;
+    explicit PoolScale(float s) : scale(s), inverse(1.0f / s) {}
+    PoolScale() {}
+    template <typename KV>
+    __device__ __forceinline__ float down(float x) const
+    {
+        return sizeof(KV) < 4 ? x * inverse : scale == 1.0f ? x : __fdiv_rn(x, scale);
+    }
+    template <typename KV>
+    __device__ __forceinline__ float4 down4(float4 v) const
+    {
+        return make_float4(down<KV>(v.x), down<KV>(v.y), down<KV>(v.z), down<KV>(v.w));
+    }
+};
+
+struct AppendDev {
+    PagedDev c;
+    PoolScale k, v;
+    int page_shift;  // log2(page_size), or -1
+    int mode, n_dims, n_offs;
+    long long stride_q, stride_k, stride_v, stride_q_out;
+    int has_q;
+};
 
 // (a, b) turned by the angle of cosine c and sine s, in float64, rounded once.
 __device__ __forceinline__ void turn(float& a, float& b, double c, double s)
@@ -290,7 +305,8 @@ __device__ __forceinline__ void turn(float& a, float& b, double c, double s)
 
 // One CTA per token. The angles are formed once per token, in float64 as k_kv_append forms them, and shared by its
 // heads. V4: a thread's unit is two float4 of a row - four pairs, or eight channels that pass unchanged, or eight
-// channels of v - all loaded before the angles are waited for; else a unit is one pair. Bound by the bytes
+// channels of v, the second float4 half a range behind the first so that neighbours' accesses join up - all loaded
+// before the angles are waited for; else a unit is one pair. Bound by the bytes
 // (q twice, k and v once, the pools' rows): 6001 tokens of 32/8 heads of 128 into an e4m3 pool, 259 MB, take 55 us (4.7
 // TB/s, 0.72 of the copy rate); the float64 rotation costs 1.5 us of it. A CTA that takes several tokens with the next
 // one's loads under way was slower (63 us in registers, 97 us through shared memory): CTAs of one token are dealt out as
@@ -311,7 +327,7 @@ __global__ void __launch_bounds__(kAppendThreads, 4) k_paged_append(AppendDev p,
     if (slot < 0 || slot >= p.c.page_size * p.c.num_pages)
         return;
     const int half = p.n_dims / 2, hd = p.c.head_dim;
-    const int page = slot / p.c.page_size, at = slot - page * p.c.page_size;
+    const int page = p.page_shift >= 0 ? slot >> p.page_shift : slot / p.c.page_size, at = slot - page * p.c.page_size;
     const long long row = page * p.c.page_stride + at * p.c.slot_stride;
     const int heads = p.has_q ? p.c.heads : 0;
     const auto angles = [&]() {
@@ -324,7 +340,7 @@ __global__ void __launch_bounds__(kAppendThreads, 4) k_paged_append(AppendDev p,
         }
     };
     if constexpr (V4) {
-        const int per_head = hd / 8, turned = p.n_dims / 8;  // units
+        const int shift = __ffs(hd) - 4, per_head = hd / 8, turned = p.n_dims / 8;  // units; hd is a power of two
         const int qk = (heads + p.c.kv_heads) * per_head, all = qk + p.c.kv_heads * per_head;
         constexpr int U = 3;  // a thread's units at a time
         bool formed = false;
@@ -336,14 +352,13 @@ __global__ void __launch_bounds__(kAppendThreads, 4) k_paged_append(AppendDev p,
             for (int i = 0; i < U; ++i) {
                 const int e = base + i * kAppendThreads;
                 if (e < all) {
-                    const int h = e / per_head, u = e - h * per_head;
+                    const int h = e >> shift, u = e & (per_head - 1);
                     if (e >= qk) {
-                        d0[i] = 8 * u, d1[i] = 8 * u + 4;
+                        d0[i] = 4 * u, d1[i] = d0[i] + hd / 2;
                     } else if (u < turned) {
-                        d0[i] = p.n_offs + (p.mode == MUYO_ROPE_NEOX ? 4 * u : 8 * u);
-                        d1[i] = d0[i] + (p.mode == MUYO_ROPE_NEOX ? half : 4);
+                        d0[i] = p.n_offs + 4 * u, d1[i] = d0[i] + half;
                     } else {
-                        d0[i] = 8 * (u - turned), d1[i] = d0[i] + 4;
+                        d0[i] = 4 * (u - turned), d1[i] = d0[i] + (hd - p.n_dims) / 2;
                         d0[i] += d0[i] < p.n_offs ? 0 : p.n_dims;
                         d1[i] += d1[i] < p.n_offs ? 0 : p.n_dims;
                     }
@@ -363,12 +378,16 @@ __global__ void __launch_bounds__(kAppendThreads, 4) k_paged_append(AppendDev p,
             for (int i = 0; i < U; ++i) {
                 const int e = base + i * kAppendThreads;
                 if (e < all) {
-                    const int h = e / per_head, u = e - h * per_head;
+                    const int h = e >> shift, u = e & (per_head - 1);
                     if (e < qk && u < turned) {
-                        const double2* c = reinterpret_cast<const double2*>(cs + 4 * u);
-                        const double2* s = reinterpret_cast<const double2*>(cs + half + 4 * u);
-                        const double2 c0 = c[0], c1 = c[1], s0 = s[0], s1 = s[1];
-                        if (p.mode == MUYO_ROPE_NEOX) {
+                        // the pairs in a row: 4 u .. 4 u + 3, or 2 u, 2 u + 1 and those half / 2 behind them
+                        const bool neox = p.mode == MUYO_ROPE_NEOX;
+                        const int at = neox ? 4 * u : 2 * u, next = neox ? at + 2 : at + half / 2;
+                        const double2 c0 = *reinterpret_cast<const double2*>(cs + at);
+                        const double2 c1 = *reinterpret_cast<const double2*>(cs + next);
+                        const double2 s0 = *reinterpret_cast<const double2*>(cs + half + at);
+                        const double2 s1 = *reinterpret_cast<const double2*>(cs + half + next);
+                        if (neox) {
                             turn(x[i][0].x, x[i][1].x, c0.x, s0.x);
                             turn(x[i][0].y, x[i][1].y, c0.y, s0.y);
                             turn(x[i][0].z, x[i][1].z, c1.x, s1.x);
@@ -387,9 +406,9 @@ __global__ void __launch_bounds__(kAppendThreads, 4) k_paged_append(AppendDev p,
                     } else {
                         const bool is_v = e >= qk;
                         KV* y = (is_v ? v_pool : k_pool) + row + (h - heads - (is_v ? p.c.kv_heads : 0)) * p.c.head_stride;
-                        const float scale = is_v ? p.c.v_scale : p.c.k_scale;
-                        pool_store4<KV>(y + d0[i], scaled_down(x[i][0], scale));
-                        pool_store4<KV>(y + d1[i], scaled_down(x[i][1], scale));
+                        const PoolScale scale = is_v ? p.v : p.k;
+                        pool_store4<KV>(y + d0[i], scale.down4<KV>(x[i][0]));
+                        pool_store4<KV>(y + d1[i], scale.down4<KV>(x[i][1]));
                     }
                 }
             }
@@ -421,13 +440,13 @@ __global__ void __launch_bounds__(kAppendThreads, 4) k_paged_append(AppendDev p,
                 y[j1] = y1;
             } else {
                 KV* y = k_pool + row + (h - heads) * p.c.head_stride;
-                y[j0] = pool_round<KV>(__fdiv_rn(y0, p.c.k_scale));
-                y[j1] = pool_round<KV>(__fdiv_rn(y1, p.c.k_scale));
+                y[j0] = pool_round<KV>(p.k.down<KV>(y0));
+                y[j1] = pool_round<KV>(p.k.down<KV>(y1));
             }
         }
         for (int e = tid; e < p.c.kv_heads * hd; e += kAppendThreads) {
             const int h = e / hd, d = e - h * hd;
-            v_pool[row + h * p.c.head_stride + d] = pool_round<KV>(__fdiv_rn(v[t * p.stride_v + e], p.c.v_scale));
+            v_pool[row + h * p.c.head_stride + d] = pool_round<KV>(p.v.down<KV>(v[t * p.stride_v + e]));
         }
     }
 }
@@ -534,6 +553,8 @@ extern "C" int muyo_cuda_paged_rope_append(const MuyoPagedAppendParams* p, const
     MUYO_REQUIRE((d.stride_q | d.stride_k | d.stride_v | d.stride_q_out) % 4 == 0,
                  "paged_rope_append: row strides must be multiples of 4");
     MUYO_REQUIRE(q != q_out || !q || d.stride_q == d.stride_q_out, "paged_rope_append: q in place needs equal strides");
+    d.k = PoolScale(d.c.k_scale), d.v = PoolScale(d.c.v_scale);
+    d.page_shift = page_shift_of(d.c.page_size);
     d.mode = (int)p->rope_mode, d.n_dims = (int)p->n_dims, d.n_offs = (int)p->n_offs, d.has_q = q != nullptr;
     if (p->tokens == 0)
         return MUYO_OK;

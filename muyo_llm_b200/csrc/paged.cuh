@@ -35,8 +35,8 @@ inline int paged_prepare(const MuyoPagedCache& c, const char* what, PagedDev& d)
     MUYO_REQUIRE(c.page_size > 0 && c.num_pages > 0, "%s: page_size and num_pages must be positive", what);
     MUYO_REQUIRE((uint64_t)c.page_size * c.num_pages <= (uint64_t)INT_MAX, "%s: %u pages of %u slots exceed INT32_MAX slots",
                  what, c.num_pages, c.page_size);
-    MUYO_REQUIRE(std::isfinite(c.k_scale) && std::isfinite(c.v_scale) && c.k_scale >= 0.0f && c.v_scale >= 0.0f,
-                 "%s: k_scale and v_scale must be finite and not negative", what);
+    const auto fits = [](float s) { return s == 0.0f || (s >= 0x1p-100f && s <= 0x1p100f); };
+    MUYO_REQUIRE(fits(c.k_scale) && fits(c.v_scale), "%s: k_scale and v_scale must be 0 or in [2^-100, 2^100]", what);
     d.heads = (int)c.heads, d.kv_heads = (int)c.kv_heads, d.group = (int)(c.heads / c.kv_heads);
     d.head_dim = (int)c.head_dim, d.page_size = (int)c.page_size, d.num_pages = (int)c.num_pages;
     d.k_scale = c.k_scale == 0.0f ? 1.0f : c.k_scale;

@@ -42,6 +42,8 @@ BAD_CACHES = [
     (EINVAL, dict(page_size=1 << 16, num_pages=1 << 15), "INT32_MAX"),
     (EINVAL, dict(k_scale=-1.0), "k_scale"),
     (EINVAL, dict(v_scale=float("inf")), "v_scale"),
+    (EINVAL, dict(k_scale=2.0 ** -101), "k_scale"),
+    (EINVAL, dict(v_scale=2.0 ** 101), "v_scale"),
     (EINVAL, dict(page_stride=64, head_stride=64, slot_stride=32), "below head_dim"),
     (EINVAL, dict(page_stride=4096), "below head_dim"),  # all three strides or none
     (EINVAL, dict(page_stride=4100, head_stride=64, slot_stride=64), "16 bytes"),
