@@ -307,14 +307,15 @@ __device__ __forceinline__ void turn(float& a, float& b, double c, double s)
 // heads. V4: a thread's unit is two float4 of a row - four pairs, or eight channels that pass unchanged, or eight
 // channels of v, the second float4 half a range behind the first so that neighbours' accesses join up - all loaded
 // before the angles are waited for; else a unit is one pair. Bound by the bytes
-// (q twice, k and v once, the pools' rows): 6001 tokens of 32/8 heads of 128 into an e4m3 pool, 259 MB, take 55 us (4.7
-// TB/s, 0.72 of the copy rate); the float64 rotation costs 1.5 us of it. A CTA that takes several tokens with the next
-// one's loads under way was slower (63 us in registers, 97 us through shared memory): CTAs of one token are dealt out as
-// SMs come free.
-constexpr int kAppendThreads = 256;
+// (q twice, k and v once, the pools' rows): 6001 tokens of 32/8 heads of 128 into an e4m3 pool, 259 MB, take 43.4 us (6.0
+// TB/s, 0.91 of the copy rate); the float64 rotation costs 2 us of it. Eight CTAs of four warps on an SM keep loads, turns and
+// stores of different tokens going side by side: four of eight warps take 46.8 us, and a CTA that takes several tokens
+// with the next one's loads under way more (63 us in registers, 97 us through shared memory): CTAs of one token are
+// dealt out as SMs come free.
+constexpr int kAppendThreads = 128;
 
 template <typename KV, bool V4>
-__global__ void __launch_bounds__(kAppendThreads, 4) k_paged_append(AppendDev p, const float* q, const float* k, const float* v,
+__global__ void __launch_bounds__(kAppendThreads, 8) k_paged_append(AppendDev p, const float* q, const float* k, const float* v,
                                                                  const int32_t* positions, const int32_t* slots,
                                                                  const double* __restrict__ freqs, float* q_out, KV* k_pool,
                                                                  KV* v_pool)
@@ -344,6 +345,11 @@ __global__ void __launch_bounds__(kAppendThreads, 4) k_paged_append(AppendDev p,
         const int qk = (heads + p.c.kv_heads) * per_head, all = qk + p.c.kv_heads * per_head;
         constexpr int U = 3;  // a thread's units at a time
         bool formed = false;
+        // so that head h of the CTA's heads (q's, k's, v's) is h * hd behind its row
+        const float* q_row = q + t * p.stride_q;
+        const float* k_row = k + t * p.stride_k - heads * hd;
+        const float* v_row = v + t * p.stride_v - (heads + p.c.kv_heads) * hd;
+        float* q_out_row = q_out + t * p.stride_q_out;
 #pragma unroll 1
         for (int base = tid; base - tid < all; base += U * kAppendThreads) {
             float4 x[U][2];
@@ -362,9 +368,7 @@ __global__ void __launch_bounds__(kAppendThreads, 4) k_paged_append(AppendDev p,
                         d0[i] += d0[i] < p.n_offs ? 0 : p.n_dims;
                         d1[i] += d1[i] < p.n_offs ? 0 : p.n_dims;
                     }
-                    const float* src = e >= qk ? v + t * p.stride_v + (long long)(h - heads - p.c.kv_heads) * hd
-                                       : h < heads ? q + t * p.stride_q + (long long)h * hd
-                                                   : k + t * p.stride_k + (long long)(h - heads) * hd;
+                    const float* src = (e >= qk ? v_row : h < heads ? q_row : k_row) + (h << (shift + 3));
                     x[i][0] = *reinterpret_cast<const float4*>(src + d0[i]);
                     x[i][1] = *reinterpret_cast<const float4*>(src + d1[i]);
                 }
@@ -400,7 +404,7 @@ __global__ void __launch_bounds__(kAppendThreads, 4) k_paged_append(AppendDev p,
                         }
                     }
                     if (h < heads) {
-                        float* y = q_out + t * p.stride_q_out + (long long)h * hd;
+                        float* y = q_out_row + (h << (shift + 3));
                         *reinterpret_cast<float4*>(y + d0[i]) = x[i][0];
                         *reinterpret_cast<float4*>(y + d1[i]) = x[i][1];
                     } else {
