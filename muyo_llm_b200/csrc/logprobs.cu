@@ -12,8 +12,10 @@ namespace cg = cooperative_groups;
 
 namespace muyo {
 
-constexpr int kLogprobThreads = 256;
-constexpr int kLogprobWarps = kLogprobThreads / 32;
+// With alternatives a thread's part of a row is what is read again, and fewer threads would have longer ones; without,
+// more and smaller CTAs on an SM begin and end beside the others' loops (2001 rows of 32001: 53.1 us, 256 threads 56.8).
+template <bool TOP>
+constexpr int kLogprobThreads = TOP ? 256 : 128;
 constexpr int kLogprobJoinThreads = 128;
 constexpr int kLogprobMaxTop = 32;
 constexpr int kLogprobGroups = 64;  // groups of 4 threads whose maxima give the threshold
@@ -179,14 +181,15 @@ __device__ __forceinline__ LogprobPiece logprob_join_sums(const LogprobDev& p, L
 // loop ends at 40% of the kernel's time, the rest is the second reads and the cluster's join), one row 8.5 us. Listing
 // tile by tile in the loop took 40 us for the 97 rows, whole pieces in shared memory 59 us.
 template <bool TOP, int V>
-__global__ void __launch_bounds__(kLogprobThreads, 4) k_logprob_pieces(LogprobDev p, const float* logits,
+__global__ void __launch_bounds__(kLogprobThreads<TOP>, 1024 / kLogprobThreads<TOP>)
+                                                      k_logprob_pieces(LogprobDev p, const float* logits,
                                                                        const int32_t* tokens,
                                                                        LogprobPiece* stats,
                                                                        unsigned long long* tops, LogprobOut out)
 {
-    constexpr int WARPS = kLogprobWarps, Q = kLogprobThreads * 4, TILE = V * Q;
-    __shared__ float s_m[WARPS], s_r[WARPS], s_e[WARPS], s_mine[TOP ? kLogprobThreads : 1], s_threshold;
-    __shared__ int s_before[WARPS], s_count, s_threads, s_thread[TOP ? kLogprobThreads : 1];
+    constexpr int THREADS = kLogprobThreads<TOP>, WARPS = THREADS / 32, Q = THREADS * 4, TILE = V * Q;
+    __shared__ float s_m[WARPS], s_r[WARPS], s_e[WARPS], s_mine[TOP ? THREADS : 1], s_threshold;
+    __shared__ int s_before[WARPS], s_count, s_threads, s_thread[TOP ? THREADS : 1];
     __shared__ unsigned long long s_key[WARPS], s_top[kLogprobMaxTop], s_list[TOP ? kLogprobList : 1];
     __shared__ LogprobPiece s_sum;
     pdl_wait();
@@ -376,7 +379,7 @@ __global__ void __launch_bounds__(kLogprobThreads, 4) k_logprob_pieces(LogprobDe
             s_top[tid] = 0ull;
         __syncthreads();
 #pragma unroll 1
-        for (int k = tid; k < n; k += kLogprobThreads) {
+        for (int k = tid; k < n; k += THREADS) {
             const unsigned long long key = s_list[k];
             int place = 0;
 #pragma unroll 8
@@ -458,7 +461,7 @@ __global__ void __launch_bounds__(kLogprobThreads, 4) k_logprob_pieces(LogprobDe
             for (int k = 0; k < p.top_k; ++k) {
                 unsigned long long next = 0ull;
 #pragma unroll 4
-                for (int i = begin + tid; i < end; i += kLogprobThreads) {
+                for (int i = begin + tid; i < end; i += THREADS) {
                     const float y = x[i];
                     const unsigned long long key = y > -INFINITY ? order_key(y, i) : 0ull;
                     next = key < last && key > next ? key : next;
@@ -608,6 +611,8 @@ __global__ void __launch_bounds__(kLogprobJoinThreads) k_logprob_join(LogprobDev
 
 using namespace muyo;
 
+static int logprob_threads(const LogprobDev& d) { return d.top_k > 0 ? kLogprobThreads<true> : kLogprobThreads<false>; }
+
 static int logprobs_prepare(const MuyoTokenLogprobsParams* p, LogprobDev& d)
 {
     MUYO_REQUIRE(p, "token_logprobs: null parameter block");
@@ -626,10 +631,11 @@ static int logprobs_prepare(const MuyoTokenLogprobsParams* p, LogprobDev& d)
     // us, 3 pieces 34 us), and not into more than a cluster joins where those are a CTA per SM (40 rows: 8 pieces 20
     // us, 14 pieces and a second kernel 22 us; one row: 8 pieces 13 us, 75 pieces 8 us). A row may begin 3 logits
     // behind a 16-byte border.
-    const long long large = (d.vocab + 3LL + 16 * kLogprobThreads - 1) / (16 * kLogprobThreads);
+    const int threads = logprob_threads(d), per_sm = 768 / threads;
+    const long long large = (d.vocab + 3LL + 16 * threads - 1) / (16 * threads);
     d.small = large * d.rows < sm_count();  // the larger tiles would leave SMs without a CTA
-    const long long tiles = d.small ? (d.vocab + 3LL + 8 * kLogprobThreads - 1) / (8 * kLogprobThreads) : large;
-    long long cut = std::max(1LL, std::min((3LL * sm_count() + d.rows / 2) / d.rows, tiles));
+    const long long tiles = d.small ? (d.vocab + 3LL + 8 * threads - 1) / (8 * threads) : large;
+    long long cut = std::max(1LL, std::min(((long long)per_sm * sm_count() + d.rows / 2) / d.rows, tiles));
     if (cut > kLogprobCluster && d.rows * (long long)kLogprobCluster >= sm_count())
         cut = kLogprobCluster;
     const long long each = std::min((tiles + cut - 1) / cut, (long long)kLogprobMaxTiles);
@@ -676,7 +682,7 @@ extern "C" int muyo_cuda_token_logprobs(const MuyoTokenLogprobsParams* p, const 
                                 : (d.top_k > 0 ? k_logprob_pieces<true, 4> : k_logprob_pieces<false, 4>);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(d.rows * d.pieces);
-    cfg.blockDim = dim3(kLogprobThreads);
+    cfg.blockDim = dim3(logprob_threads(d));
     cfg.stream = as_stream(stream);
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
