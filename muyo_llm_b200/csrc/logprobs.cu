@@ -13,7 +13,7 @@ namespace cg = cooperative_groups;
 namespace muyo {
 
 // With alternatives a thread's part of a row is what is read again, and fewer threads would have longer ones; without,
-// more and smaller CTAs on an SM begin and end beside the others' loops (2001 rows of 32001: 53.1 us, 256 threads 56.8).
+// more and smaller CTAs on an SM begin and end beside the others' loops (2001 rows of 32001: 53.1 us, with 256 threads 56.8 us).
 template <bool TOP>
 constexpr int kLogprobThreads = TOP ? 256 : 128;
 constexpr int kLogprobJoinThreads = 128;
@@ -76,9 +76,7 @@ __device__ __forceinline__ unsigned long long warp_max_key(unsigned long long v)
 constexpr float kLogprobDown = 5.421010862427522e-20f;  // 2^-64
 __device__ __forceinline__ float weight_up(float u, float inv_t)
 {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fmaf(u, inv_t, 64.0f)));
-    return y;
+    return ex2(fmaf(u, inv_t, 64.0f));
 }
 constexpr float kLogprobLeast = -1.0e29f;  // u where the weight is 0, so that 0 * -inf does not arise
 
@@ -176,8 +174,9 @@ __device__ __forceinline__ LogprobPiece logprob_join_sums(const LogprobDev& p, L
 // constant row, a mask of the lowest value) run the list over: then what lies above it is listed, and of the equal
 // ones the lowest ids.
 //
-// Bound by the read, 4 bytes a logit: 2001 rows of 32001, 256 MB, take 56 us (4.6 TB/s, 0.70 of the copy rate; a CTA's
-// first loads and its last sums are a third of its time), 97 rows of 151936 with 20 alternatives, 59 MB, 23.5 us (the
+// Bound by the read, 4 bytes a logit: 2001 rows of 32001, 256 MB, take 51 us (5.0 TB/s, 0.76 of the copy rate; a CTA's
+// first loads and its last sums are a third of its time, the count for the rank 2 us and the entropy's sum 3 us of the
+// call), 97 rows of 151936 with 20 alternatives, 59 MB, 23.2 us (the
 // loop ends at 40% of the kernel's time, the rest is the second reads and the cluster's join), one row 8.5 us. Listing
 // tile by tile in the loop took 40 us for the 97 rows, whole pieces in shared memory 59 us.
 template <bool TOP, int V>
@@ -237,7 +236,7 @@ __global__ void __launch_bounds__(kLogprobThreads<TOP>, 1024 / kLogprobThreads<T
     // not masked. The four logits around the token have both kinds: put right after the loop.
     const float below = xt == -INFINITY ? INFINITY : nextafterf(xt, -INFINITY);
     float m = -INFINITY, r = 0.0f, e = 0.0f;  // r, e: 2^64 times the sums
-    int before = 0;
+    float front = 0.0f;  // ids in front of the token: exact, a thread has 1024 logits of a piece at most
     if (tid == 0)
         s_count = s_threads = 0;
     const auto work = [&](const float4 (&v)[V], int tile) {
@@ -246,16 +245,18 @@ __global__ void __launch_bounds__(kLogprobThreads<TOP>, 1024 / kLogprobThreads<T
         for (int j = 1; j < V; ++j)
             mine = fmaxf(fmaxf(mine, fmaxf(v[j].x, v[j].y)), fmaxf(v[j].z, v[j].w));
         const float mn = fmaxf(m, mine), ms = mn == -INFINITY ? 0.0f : mn;
-        float tr = 0.0f, te = 0.0f;
+        const float2 scale = make_float2(p.inv_t, p.inv_t), up = make_float2(64.0f, 64.0f), back = make_float2(-ms, -ms);
+        float2 sum = make_float2(0.0f, 0.0f), moment = sum;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const float u0 = v[j].x - ms, u1 = v[j].y - ms, u2 = v[j].z - ms, u3 = v[j].w - ms;
-            const float w0 = weight_up(u0, p.inv_t), w1 = weight_up(u1, p.inv_t), w2 = weight_up(u2, p.inv_t),
-                        w3 = weight_up(u3, p.inv_t);
-            tr += (w0 + w1) + (w2 + w3);
-            te = fmaf(w0, fmaxf(u0, kLogprobLeast), te), te = fmaf(w1, fmaxf(u1, kLogprobLeast), te);
-            te = fmaf(w2, fmaxf(u2, kLogprobLeast), te), te = fmaf(w3, fmaxf(u3, kLogprobLeast), te);
+            const float2 u0 = add2(make_float2(v[j].x, v[j].y), back), u1 = add2(make_float2(v[j].z, v[j].w), back);
+            const float2 x0 = fma2(u0, scale, up), x1 = fma2(u1, scale, up);  // as in weight_up
+            const float2 w0 = make_float2(ex2(x0.x), ex2(x0.y)), w1 = make_float2(ex2(x1.x), ex2(x1.y));
+            sum = add2(sum, add2(w0, w1));
+            moment = fma2(w0, make_float2(fmaxf(u0.x, kLogprobLeast), fmaxf(u0.y, kLogprobLeast)), moment);
+            moment = fma2(w1, make_float2(fmaxf(u1.x, kLogprobLeast), fmaxf(u1.y, kLogprobLeast)), moment);
         }
+        const float tr = sum.x + sum.y, te = moment.x + moment.y;
         // the sums so far, relative to the new largest (at 0 before the first logit above -inf)
         const float u = fmaxf(m - ms, kLogprobLeast), w = weight_up(u, p.inv_t) * kLogprobDown;
         e = w > 0.0f ? fmaf(w, fmaf(u, r, e), te) : te;  // u * r is finite where w is not 0
@@ -266,7 +267,8 @@ __global__ void __launch_bounds__(kLogprobThreads<TOP>, 1024 / kLogprobThreads<T
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 const float border = i + j * Q + 3 < token ? below : xt;
-                before += (v[j].x > border) + (v[j].y > border) + (v[j].z > border) + (v[j].w > border);
+                front += ((v[j].x > border ? 1.0f : 0.0f) + (v[j].y > border ? 1.0f : 0.0f)) +
+                         ((v[j].z > border ? 1.0f : 0.0f) + (v[j].w > border ? 1.0f : 0.0f));
             }
         }
     };
@@ -281,6 +283,7 @@ __global__ void __launch_bounds__(kLogprobThreads<TOP>, 1024 / kLogprobThreads<T
             work(vb, tile + 1);
         }
     }
+    int before = (int)front;
     if (tid == 0) {
         if (token >= begin && token < end) {
 #pragma unroll 1

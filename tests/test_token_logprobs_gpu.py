@@ -2,8 +2,8 @@
 
 Tolerances, u = 2^-24: with d = (x - m) / T and w = exp(d), a term's relative error is at most (3 |d| + 8) u (the
 difference, the scaling and the exponential), and a sum over the row adds at most 128 u (the longest chain of
-additions: 7 in a tile of a thread, up to 64 tiles, 5 and 3 levels in a block, up to 8 pieces in a thread of the join
-and its 7 levels: 94). The largest's own 1 is exact. So
+additions: 9 in a tile of a thread, up to 64 tiles, 5 and 3 levels in a block, up to 8 pieces in a thread of the join
+and its 7 levels: 96). The largest's own 1 is exact. So
 log(1 + R) is off by at most u sum_others p (3 |d| + 136) and a log probability by that and 3 u |x - m| / T of the
 subtraction and the division; entropy's second sum weighs each term by |d| again. Ids, ranks and their order are exact.
 """
