@@ -632,8 +632,8 @@ static int logprobs_prepare(const MuyoTokenLogprobsParams* p, LogprobDev& d)
     // A row is cut into the pieces that come nearest to three CTAs on an SM (97 rows of 151936 with 20 alternatives: 5
     // pieces 23.5 us, 6 pieces 30 us, the ends of more pieces cost more than their loops gain; 150 rows: 2 pieces 44
     // us, 3 pieces 34 us), and not into more than a cluster joins where those are a CTA per SM (40 rows: 8 pieces 20
-    // us, 14 pieces and a second kernel 22 us; one row: 8 pieces 13 us, 75 pieces 8 us). A row may begin 3 logits
-    // behind a 16-byte border.
+    // us, 14 pieces and a second kernel 22 us; one row: 8 pieces 13 us, 75 pieces 8 us); of the smaller CTAs, as many as
+    // fill the same threads. A row may begin 3 logits behind a 16-byte border.
     const int threads = logprob_threads(d), per_sm = 768 / threads;
     const long long large = (d.vocab + 3LL + 16 * threads - 1) / (16 * threads);
     d.small = large * d.rows < sm_count();  // the larger tiles would leave SMs without a CTA

@@ -19,8 +19,8 @@
 //
 // Measured: 131071 keys of 32/8 heads of 128 in F16, 537 MB, 99 us (5.4 TB/s, 0.83 of the copy rate; the SMs of some
 // GPCs stream 12% slower than the others, and even shares wait for them); 64 requests over 2000 to 16000 e4m3 keys,
-// 901 MB, 187 us (4.8 TB/s, 0.74; the conversions' dependent chains with 8 warps on an SM - twice the warps with tiles of
-// half the size: 214 us); 200 requests over 60 to 2048 keys of 14/2 heads of 64 in F16, 60 MB, 23 us (start, joins and
+// 901 MB, 175 us (5.1 TB/s, 0.78; the conversions' dependent chains with 8 warps on an SM - 12 warps with tiles of half
+// the size take an eighth more); 200 requests over 60 to 2048 keys of 14/2 heads of 64 in F16, 60 MB, 23 us (start, joins and
 // the second kernel are two thirds); one request over 1023 keys 8.4 us (two launches); 33 requests of 16 heads on one
 // F32 head, windows of 4096 keys, 80 MB, 42 us (the splitting of F32 operands).
 //
@@ -65,8 +65,8 @@ struct PagedTile {
     static constexpr int RB = HD * ES;        // bytes of a row
     static constexpr int CPR = RB / 16;       // 16-byte chunks of a row
     static constexpr int KSTEP = T == MUYO_KV_F32 ? 8 : 16;
-    // 4 KB of keys: half of that with three CTAs on an SM took 214 us where this takes 190 (64 requests, e4m3). At most
-    // 64: a warp votes and masks two keys a lane.
+    // 4 KB of keys: half of that with three CTAs on an SM took 214 us where 4 KB took 190 (64 requests, e4m3). At most
+    // 64 keys: a warp votes and masks two keys a lane.
     static constexpr int KT = kPagedTile / RB > 64 ? 64 : kPagedTile / RB < KSTEP ? KSTEP : kPagedTile / RB;  // keys of a tile
     static constexpr int STAGES = WIDE ? 2 : 3;  // WIDE: a third would leave shared memory for one CTA
     static constexpr int TILE = KT * RB;      // bytes of a tile's keys (or values)
