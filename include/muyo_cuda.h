@@ -520,9 +520,8 @@ int muyo_cuda_rope_frequencies(const MuyoRopeParams* p, const float* freq_factor
  * angles, rotation in float64 rounded once, as muyo_cuda_kv_append): NEOX pairs channels
  * (j, j + n_dims/2), NORMAL pairs (2j, 2j + 1), of the n_dims channels from n_offs; the others pass
  * unchanged. The turned q goes to q_out (which may be q with the same stride), the turned k and the
- * v, divided by their scales (F16 and F8: times the scale's F32 reciprocal) and rounded to the pool's
- * type, to slot slots[t] of their pools. A token
- * with a slot outside [0, num_pages * page_size) is left out: no q_out row, no pool is written.
+ * v, divided by their scales (rounded to F32) and rounded to the pool's type, to slot slots[t] of their
+ * pools. A token with a slot outside [0, num_pages * page_size) is left out: no q_out row, no pool is written.
  * Slots of one call must differ from one another: of two tokens in one slot either may stay, channel
  * by channel. q may be NULL (keys and values only). n_dims 0 turns nothing and reads no freqs. */
 typedef struct MuyoPagedAppendParams {

@@ -1,0 +1,67 @@
+"""Paged-cache entry points at the ends of their ranges: stored values next to a rounding border, scores far beyond
+the weights' range, batches around the default limit of shared memory, rows of the most slots, a step as a host drives it.
+
+U = 2^-24, half a step of F32."""
+from __future__ import annotations
+
+import math
+import os
+import subprocess
+import sys
+
+import numpy as np
+import pytest
+import torch
+
+from conftest import ROOT
+from muyo_llm_b200 import _abi, nodes
+from test_paged_gpu import DTYPES, Server, as_bits, attention64, gen, ints, plan_reference, randn, rotated64, run_plan
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+# ---- stored values ------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("n_dims,n_offs", [(0, 0), (6, 2)])  # units of two float4, and pairs
+@pytest.mark.parametrize("dtype", [_abi.KV_F32, _abi.KV_F16, _abi.KV_F8])
+@pytest.mark.parametrize("scale", [0.03, 0.02, 1.0 / 3.0, 0.7, 3.0, 1.0, 2.0 ** -99 * 1.5, 1e20])
+def test_append_stores_the_quotient(cuda, dtype, scale, n_dims, n_offs):
+    """Every value next to a border of e4m3's or F16's rounding, bit for bit: x / scale rounded to F32, then to the pool's
+    type (to e4m3: at most +-448). Both roundings are of the quotient, so there is no tolerance."""
+    kv, hd, page = 2, 64, 16
+    s = np.float32(scale)
+    steps = torch.arange(0x7F, dtype=torch.uint8).view(torch.float8_e4m3fn).float().numpy()
+    if dtype == _abi.KV_F16:
+        steps = np.concatenate([steps, np.arange(0x3C00, 0x3C00 + 600, dtype=np.uint16).view(np.float16).astype(np.float32)])
+    mid = ((steps[1:].astype(np.float64) + steps[:-1]) / 2 * float(s)).astype(np.float32)
+    near, up, down = [mid], mid, mid
+    for _ in range(3):
+        up, down = np.nextafter(up, np.float32(np.inf)), np.nextafter(down, np.float32(-np.inf))
+        near += [up, down]
+    x = np.concatenate(near + [np.array([0.0, np.inf, np.finfo(np.float32).max, np.nan], np.float32)])
+    x = np.concatenate([x, -x])
+    tokens = -(-len(x) // (kv * hd))
+    x = np.concatenate([x, np.zeros(tokens * kv * hd - len(x), np.float32)])
+    with np.errstate(over="ignore", invalid="ignore"):
+        q = torch.from_numpy(x / s).reshape(tokens, kv, hd)
+    want = as_bits((q.clamp(-448, 448) if dtype == _abi.KV_F8 else q).to(DTYPES[dtype]))
+    pages = -(-tokens // page)
+    cache = nodes.paged_cache_params(kv, kv, hd, page_size=page, num_pages=pages, kv_dtype=dtype, order="nhd", k_scale=scale, v_scale=scale)
+    pools = [torch.zeros((pages * page, kv, hd), device="cuda").to(DTYPES[dtype]) for _ in range(2)]
+    xd, at = torch.from_numpy(x).cuda(), torch.arange(tokens, dtype=torch.int32, device="cuda")
+    freqs = torch.zeros(n_dims // 2 + 1, dtype=torch.float64, device="cuda")
+    freqs[-1] = 1.0  # turned by nothing: x cos 0 - y sin 0 is x for finite x and y
+    nodes.paged_rope_append(nodes.paged_append_params(cache, tokens, n_dims=n_dims, n_offs=n_offs), None, xd, xd, torch.zeros_like(at), at,
+                            freqs, None, *pools)
+    torch.cuda.synchronize()
+    for name, pool in zip("kv", pools):
+        got = as_bits(pool.cpu())[:tokens]
+        keep = torch.ones(hd, dtype=torch.bool)
+        if name == "k":
+            keep[n_offs:n_offs + n_dims] = False  # infinities meet zeros there
+        if dtype == _abi.KV_F8:
+            same = (got == want) | ((got & 0x7F == 0x7F) & (want & 0x7F == 0x7F))
+        else:
+            same = (got == want) | (torch.isnan(got) & torch.isnan(want))
+        assert bool(same[..., keep].all()), (name, int((~same[..., keep]).sum()))
