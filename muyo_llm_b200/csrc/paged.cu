@@ -490,8 +490,8 @@ extern "C" int muyo_cuda_paged_plan(const MuyoPagedPlanParams* p, const int32_t*
                     page_shift_of((int)p->page_size)};
     const size_t smem = (size_t)p->seqs * 4 * sizeof(int);
     static std::atomic<unsigned long long> allowed{0};
-    if (smem > 48 * 1024)
-        MUYO_CUDA_TRY(allow_smem(k_paged_plan, (size_t)kPlanMaxSeqs * 4 * sizeof(int), allowed));
+    // for every size: the limit without it, 48 KB, holds for static and dynamic shared memory together
+    MUYO_CUDA_TRY(allow_smem(k_paged_plan, (size_t)kPlanMaxSeqs * 4 * sizeof(int), allowed));
     MUYO_CUDA_TRY(launch_kernel(k_paged_plan, dim3(kPlanCtas), dim3(kPlanThreads), smem, as_stream(stream), true, d, cached_lens,
                                 new_lens, block_table, free_ring, state, seq_lens, query_start, positions, slots, state_out));
     MUYO_LAUNCH_CHECK();

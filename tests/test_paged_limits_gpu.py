@@ -65,3 +65,26 @@ def test_append_stores_the_quotient(cuda, dtype, scale, n_dims, n_offs):
         else:
             same = (got == want) | (torch.isnan(got) & torch.isnan(want))
         assert bool(same[..., keep].all()), (name, int((~same[..., keep]).sum()))
+
+
+# ---- plan -----------------------------------------------------------------------------------------------------
+
+def test_plan_around_the_default_limit_of_shared_memory(cuda):
+    """In a process of its own, smaller batches first: a larger one raises the limit for all that follow."""
+    code = """
+import torch
+from muyo_llm_b200 import _abi, nodes
+_abi.call("muyo_cuda_init", 0)
+for n in (3023, 3024, 3040, 3071, 3073):
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32, device="cuda")
+    lens, starts, positions, slots, table = i32(n), i32(n + 1), i32(n), i32(n), i32(n, 1)
+    state = torch.tensor([0, n, 0, 0], device="cuda")
+    nodes.paged_plan(nodes.paged_plan_params(n, page_size=4, num_pages=n, table_stride=1, max_tokens=n), lens, i32(n) + 1, table,
+                     torch.arange(n, dtype=torch.int32, device="cuda"), state, lens, starts, positions, slots, state)
+    assert torch.equal(slots, 4 * torch.arange(n, dtype=torch.int32, device="cuda")) and bool((lens == 1).all()), n
+    assert state.tolist() == [n, n, 0, n], n
+print("done")
+"""
+    done = subprocess.run([sys.executable, "-c", code], cwd=ROOT, env={**os.environ, "PYTHONPATH": ROOT}, capture_output=True, text=True,
+                          timeout=600)
+    assert done.returncode == 0 and "done" in done.stdout, done.stderr[-2000:]
