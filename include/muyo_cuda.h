@@ -541,8 +541,8 @@ int muyo_cuda_paged_rope_append(const MuyoPagedAppendParams* p, const float* q, 
  * [seqs][heads] F32 or NULL. A request without keys gets zeros and an lse of -inf. Lengths are clamped
  * to [0, table_stride * page_size]. Keys on a page outside [0, num_pages) are left out. What lies in
  * slots outside the attended keys is not used, NaN and infinities among it; attended keys and
- * values, and q, are finite, and those of an F32 cache below 2^80 in magnitude (weights are formed 2^15
- * times as large). One call at a time may use a workspace; it may hold anything before. */
+ * values, q and the scores are finite in F32, and those of an F32 cache below 2^80 in magnitude (weights are
+ * formed 2^15 times as large). One call at a time may use a workspace; it may hold anything before. */
 typedef struct MuyoPagedAttentionParams {
     MuyoPagedCache cache;
     uint32_t seqs;         /* at most 2^28 */

@@ -453,7 +453,7 @@ k_paged_attention(PagedAttnDev p, const float* q, const char* k_pool, const char
     // ---- the segment at hand ----
     constexpr int NQ = T == MUYO_KV_F32 ? C::NKS * 2 * HR : C::NKS * 4 * HR;
     uint32_t qf[NQ];              // fragments (F32 cache: q itself)
-    float qs[HR], m[HR], l[HR];   // m: reference of the weights, the running maximum - 15
+    float qs[HR], m[HR], l[HR];   // m: reference of the weights, the running maximum - 15 rounded up
     float o[C::VPL][2 * HR];
     bool whole = false;           // this warp has the segment from its first tile on
     float raw[HR][C::NKS * C::KPS];
@@ -634,7 +634,9 @@ k_paged_attention(PagedAttnDev p, const float* q, const char* k_pool, const char
                 most = fmaxf(most, fmaxf(s[j][2 * r], s[j][2 * r + 1]));
             most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
             most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-            const float mn = fmaxf(m[r], most - 15.0f);
+            // rounded up, so that no weight passes 2^15: from 2^24 on most - 15 is between two F32 values, and a weight of 2^16
+            // has no F16 halves
+            const float mn = fmaxf(m[r], __fsub_ru(most, 15.0f));
             const float ref = mn == -INFINITY ? 0.0f : mn;  // nothing seen yet: every weight is 2^-inf
             alpha[r] = ex2(m[r] - ref);
             m[r] = mn;

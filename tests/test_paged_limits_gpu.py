@@ -88,3 +88,50 @@ print("done")
     done = subprocess.run([sys.executable, "-c", code], cwd=ROOT, env={**os.environ, "PYTHONPATH": ROOT}, capture_output=True, text=True,
                           timeout=600)
     assert done.returncode == 0 and "done" in done.stdout, done.stderr[-2000:]
+
+
+# ---- attention ------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [_abi.KV_F32, _abi.KV_F16, _abi.KV_F8])
+@pytest.mark.parametrize("heads,kv,hd", [(8, 1, 64), (16, 1, 64), (6, 2, 128), (32, 2, 128), (12, 1, 16)])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_attention_of_scores_up_to_1e9(cuda, dtype, heads, kv, hd, sign):
+    """Scores of 1e4 to 1e9 and far apart: one key takes all weight. The output is its value, with the weight's two F16
+    halves (2^-22 of it, or 4 u), a product, a division and a sum on top: 16 u. The log-sum-exp is its score, of hd products of one sign: at
+    most (2 hd + 16) u of it, and 4 u."""
+    page, lens = 16, [1, 2, 15, 40, 700, 3000]
+    g = gen(heads + hd)
+    pages = sum(-(-n // page) for n in lens)
+    ids = torch.randperm(pages, generator=g, device="cuda").to(torch.int32)
+    table = torch.full((len(lens), -(-max(lens) // page)), -1, dtype=torch.int32, device="cuda")
+    at = 0
+    for i, n in enumerate(lens):
+        had = -(-n // page)
+        table[i, :had] = ids[at:at + had]
+        at += had
+    pattern = torch.where(torch.rand((kv, hd), generator=g, device="cuda") < 0.5, 1.0, -1.0)
+    level = torch.randint(2, 15, (pages * page,), generator=g, device="cuda").float()  # exact in e4m3
+    best = []
+    for i, n in enumerate(lens):
+        rows = table[i].long().clamp(min=0)[torch.arange(n, device="cuda") // page] * page + torch.arange(n, device="cuda") % page
+        low, high = int(rows[n // 3]), int(rows[n - 1])
+        level[low], level[high] = (1.0, 15.0) if low != high else (5.0, 5.0)
+        best.append(high if sign > 0 else low)
+    k = (level[:, None, None] * pattern).to(DTYPES[dtype])
+    v = torch.randn((pages * page, kv, hd), generator=g, device="cuda").to(DTYPES[dtype])
+    # of each head another size: scores of size * 15 at most, a step of the levels apart
+    size = torch.logspace(4, 9, len(lens) * heads, device="cuda", dtype=torch.float64).float()[torch.randperm(len(lens) * heads, generator=g, device="cuda")]
+    size = size.reshape(len(lens), heads) / 15
+    q = (size / hd)[..., None] * pattern.repeat_interleave(heads // kv, 0)
+    p = nodes.paged_attention_params(nodes.paged_cache_params(heads, kv, hd, page_size=page, num_pages=pages, kv_dtype=dtype, order="nhd"),
+                                     len(lens), table_stride=table.shape[1], scale=sign)
+    out, lse = torch.empty((len(lens), heads, hd), device="cuda"), torch.empty((len(lens), heads), device="cuda")
+    n_bytes = nodes.paged_attention_workspace_size(p)
+    nodes.paged_attention_decode(p, q.contiguous(), k.reshape(pages, page, kv, hd), v.reshape(pages, page, kv, hd), table, ints(lens), out,
+                                 torch.empty(n_bytes, dtype=torch.uint8, device="cuda"), n_bytes, lse=lse)
+    torch.cuda.synchronize()
+    for i, row in enumerate(best):
+        want = v[row].double().repeat_interleave(heads // kv, 0)
+        assert bool(((out[i].double() - want).abs() <= 16 * U * want.abs()).all()), (i, lens[i])
+        score = sign * (q[i].double() * k[row].double().repeat_interleave(heads // kv, 0)).sum(-1)
+        assert bool(((lse[i].double() - score).abs() <= (2 * hd + 20) * U * score.abs()).all()), (i, lse[i], score)
