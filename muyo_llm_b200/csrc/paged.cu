@@ -21,7 +21,7 @@ namespace muyo {
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanCtas = 8;
 constexpr int kPlanMaxSeqs = 8192;
-constexpr unsigned kPlanAdmitted = 0x80000000u, kPlanEnded = 0x40000000u, kPlanHeld = 0x3fffffffu;
+constexpr unsigned kPlanAdmitted = 0x80000000u, kPlanHeld = 0x7fffffffu;  // a row holds 2^30 tokens at most
 
 struct PlanDev {
     int seqs, page_size, num_pages, table_stride, max_tokens;
@@ -81,7 +81,8 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
     int* stop = plan_smem;          // [seqs] tokens asked for up to and with this request
     int* upto = stop + p.seqs;      // [seqs] pages needed
     int* gone = upto + p.seqs;      // [seqs] pages of ended requests
-    unsigned* held = reinterpret_cast<unsigned*>(gone + p.seqs);  // [seqs] tokens held, kPlanAdmitted
+    // [seqs] kPlanAdmitted and the tokens held before, else the tokens held after the step
+    unsigned* held = reinterpret_cast<unsigned*>(gone + p.seqs);
     __shared__ PlanSums warp_sums[32];
     __shared__ int s_taken, s_refused;
     pdl_wait();
@@ -143,7 +144,7 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
         stop[i] = saturated(run.tokens);
         upto[i] = saturated(run.pages);
         gone[i] = saturated(run.ended);
-        held[i] = (unsigned)c | (ok ? kPlanAdmitted : 0u) | (n < 0 ? kPlanEnded : 0u);
+        held[i] = ok ? (unsigned)c | kPlanAdmitted : n < 0 ? 0u : (unsigned)c;
         if (ok)
             taken = (int)run.pages;
         refused += n > 0 && !ok;
@@ -164,7 +165,7 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
     for (int i = all; i < p.seqs; i += kPlanCtas * kPlanThreads) {
         const int start = i > 0 ? stop[i - 1] : 0, c = (int)(held[i] & kPlanHeld);
         query_start[i] = start;
-        seq_lens[i] = held[i] & kPlanAdmitted ? c + stop[i] - start : held[i] & kPlanEnded ? 0 : c;
+        seq_lens[i] = held[i] & kPlanAdmitted ? c + stop[i] - start : c;
     }
     // tokens
 #pragma unroll 2

@@ -90,6 +90,21 @@ print("done")
     assert done.returncode == 0 and "done" in done.stdout, done.stderr[-2000:]
 
 
+@pytest.mark.parametrize("page,width,pages", [(1 << 29, 2, 3), (1 << 30, 1, 1)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_plan_of_rows_of_the_most_slots(cuda, page, width, pages, in_place):
+    """A full row holds 2^30 tokens: idle, refused and ended ones, one with room for a last token, lengths past the row."""
+    full = 1 << 30
+    cached = [full, full, full - 1, full, (1 << 31) - 1, 0, full - 2]
+    new = [0, 1, 1, -1, 0, -1, 3]
+    table = [[(i + j) % pages for j in range(width)] for i in range(len(cached))]
+    args = (cached, new, table, list(range(pages)), (5, 5))
+    got = run_plan(*args, page, 6, in_place)
+    want = plan_reference(*args, page, 6)
+    assert want[2] == [full, full, full, 0, full, 0, full - 2] and want[6][2] == 2
+    assert list(got) == list(want)
+
+
 # ---- attention ------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", [_abi.KV_F32, _abi.KV_F16, _abi.KV_F8])
