@@ -101,7 +101,7 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
     PlanSums mine{0, 0, 0};
     for (int i = i0; i < i1; ++i) {
         const int c = min(max(cached_lens[i], 0), row_slots), n = new_lens[i];
-        const int had = page_of(p, c + p.page_size - 1);
+        const int had = page_of(p, c + (p.page_size - 1));
         const bool fits = n > 0 && n <= row_slots - c;
         mine.tokens += max(n, 0);
         mine.pages += fits ? page_of(p, c + n - 1) + 1 - had : 0;
@@ -135,7 +135,7 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
     int taken = 0, refused = 0;
     for (int i = i0; i < i1; ++i) {
         const int c = min(max(cached_lens[i], 0), row_slots), n = new_lens[i];
-        const int had = page_of(p, c + p.page_size - 1);
+        const int had = page_of(p, c + (p.page_size - 1));
         const bool fits = n > 0 && n <= row_slots - c;
         run.tokens += max(n, 0);
         run.pages += fits ? page_of(p, c + n - 1) + 1 - had : 0;
@@ -174,7 +174,7 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
         int slot = -1, pos = 0;
         if (i < p.seqs && (held[i] & kPlanAdmitted)) {
             const int c = (int)(held[i] & kPlanHeld);
-            const int had = page_of(p, c + p.page_size - 1);
+            const int had = page_of(p, c + (p.page_size - 1));
             pos = c + t - (i > 0 ? stop[i - 1] : 0);
             const int at = page_of(p, pos);
             const int page = at < had ? table[(size_t)i * p.table_stride + at]
@@ -188,7 +188,7 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
     // pages from the ring into the tables
     for (unsigned u = all; u < (unsigned)taken; u += kPlanCtas * kPlanThreads) {
         const int k = (int)u, i = first_above(upto, p.seqs, k);
-        const int had = page_of(p, (int)(held[i] & kPlanHeld) + p.page_size - 1);
+        const int had = page_of(p, (int)(held[i] & kPlanHeld) + (p.page_size - 1));
         table[(size_t)i * p.table_stride + had + k - (i > 0 ? upto[i - 1] : 0)] = ring[ring_index(first, k, p.num_pages)];
     }
     // pages of ended requests into the ring
