@@ -494,15 +494,22 @@ typedef struct MuyoPagedCache {
  *   positions, slots [max_tokens]: of each new token; slot -1 and position 0 for tokens of a refused
  *                 request and behind the last one
  * A request that does not fit its table row, that the free pages do not suffice for, or whose tokens
- * pass max_tokens is refused as a whole: its length stays and it gets no page. Pages are counted
- * in order, so once they run out every later request that needs one is refused too.
+ * pass max_tokens is refused as a whole: its length stays and it gets no page. Pages are counted in the
+ * requests' order, those that refused requests asked for among them, and no request overtakes another:
+ * from the first one that found too few pages on, every request that asks for tokens is refused, also
+ * one that has room for them in its last page. With MUYO_PLAN_ROOM in flags those that need no page are
+ * admitted there, so that decoding goes on behind a prompt that waits for pages; those that need one
+ * still wait. The tokens of refused requests, also of those too long for their table row, keep their places in the
+ * batch (query_start) and count towards max_tokens.
  * seq_lens may be cached_lens and state_out may be state (the step in place); other buffers must not
  * overlap. With both apart, a repeated call gives the same result. Lengths outside
  * [0, table_stride * page_size] are clamped, and no content of any buffer leads out of bounds. */
+#define MUYO_PLAN_ROOM 1u
 typedef struct MuyoPagedPlanParams {
     uint32_t seqs, page_size, num_pages;
     uint32_t table_stride; /* pages of a table row; table_stride * page_size at most 2^30 */
     uint32_t max_tokens;   /* may be 0 */
+    uint32_t flags;        /* 0 or MUYO_PLAN_ROOM */
 } MuyoPagedPlanParams;
 int muyo_cuda_paged_plan(const MuyoPagedPlanParams* p, const int32_t* cached_lens, const int32_t* new_lens,
                          int32_t* block_table, int32_t* free_ring, const int64_t* state, int32_t* seq_lens,

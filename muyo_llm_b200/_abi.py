@@ -23,6 +23,7 @@ MATMUL_BIAS, MATMUL_ACCUMULATE, MATMUL_TCGEN05 = 1, 2, 4
 GLU_HALVES, GLU_SWAPPED, GLU_SPLIT = 0, 1, 2
 ROPE_NORMAL, ROPE_NEOX = 0, 2
 KV_F32, KV_F16, KV_F8 = 0, 1, 2  # KV_F8 (e4m3): paged pools only
+PLAN_ROOM = 1
 
 
 class MuyoError(RuntimeError):
@@ -100,7 +101,7 @@ class PagedCache(C.Structure):
 
 
 class PagedPlanParams(C.Structure):
-    _fields_ = _fields("seqs, page_size, num_pages, table_stride, max_tokens")
+    _fields_ = _fields("seqs, page_size, num_pages, table_stride, max_tokens, flags")
 
 
 class PagedAppendParams(C.Structure):

@@ -11,7 +11,8 @@ namespace muyo {
 // ---- plan ------------------------------------------------------------------------------------------
 // need_i = ceil((c_i + a_i) / P) - ceil(c_i / P) pages for a request that holds c_i tokens and asks for
 // a_i; with stop_i and upto_i the inclusive sums of the asked tokens and of the needed pages, request i
-// is admitted iff upto_i <= free pages and stop_i <= max_tokens. Both sums are monotone, so the pages of
+// is admitted iff upto_i <= free pages and stop_i <= max_tokens (with MUYO_PLAN_ROOM, also iff need_i = 0 and
+// stop_i <= max_tokens). Both sums are monotone, so the pages of
 // the admitted requests are a contiguous run from the ring's head, and every token and every page
 // finds its request by a binary search in the sums: all outputs are written in parallel from shared
 // memory, whatever the mix of long prompts and single tokens. A cluster of 8 CTAs shares that work; each forms
@@ -26,6 +27,7 @@ constexpr unsigned kPlanAdmitted = 0x80000000u, kPlanHeld = 0x7fffffffu;  // a r
 struct PlanDev {
     int seqs, page_size, num_pages, table_stride, max_tokens;
     int page_shift;  // log2(page_size), or -1
+    bool room;       // MUYO_PLAN_ROOM
 };
 
 struct PlanSums {
@@ -138,14 +140,16 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
         const int had = page_of(p, c + (p.page_size - 1));
         const bool fits = n > 0 && n <= row_slots - c;
         run.tokens += max(n, 0);
-        run.pages += fits ? page_of(p, c + n - 1) + 1 - had : 0;
+        const int need = fits ? page_of(p, c + n - 1) + 1 - had : 0;
+        run.pages += need;
         run.ended += n < 0 ? had : 0;
-        const bool ok = fits && run.pages <= free_pages && run.tokens <= p.max_tokens;
+        const bool pages = run.pages <= free_pages || (p.room && need == 0);
+        const bool ok = fits && pages && run.tokens <= p.max_tokens;
         stop[i] = saturated(run.tokens);
         upto[i] = saturated(run.pages);
         gone[i] = saturated(run.ended);
         held[i] = ok ? (unsigned)c | kPlanAdmitted : n < 0 ? 0u : (unsigned)c;
-        if (ok)
+        if (ok && need > 0)
             taken = (int)run.pages;
         refused += n > 0 && !ok;
     }
@@ -487,8 +491,9 @@ extern "C" int muyo_cuda_paged_plan(const MuyoPagedPlanParams* p, const int32_t*
                  "paged_plan: null buffer");
     MUYO_REQUIRE(p->max_tokens == 0 || (positions && slots), "paged_plan: positions and slots are needed with max_tokens");
     MUYO_REQUIRE(aligned_to(state, 8) && aligned_to(state_out, 8), "paged_plan: state must be 8-byte aligned");
+    MUYO_REQUIRE((p->flags & ~MUYO_PLAN_ROOM) == 0, "paged_plan: unknown flags 0x%x", p->flags);
     const PlanDev d{(int)p->seqs, (int)p->page_size, (int)p->num_pages, (int)p->table_stride, (int)p->max_tokens,
-                    page_shift_of((int)p->page_size)};
+                    page_shift_of((int)p->page_size), (p->flags & MUYO_PLAN_ROOM) != 0};
     const size_t smem = (size_t)p->seqs * 4 * sizeof(int);
     static std::atomic<unsigned long long> allowed{0};
     // for every size: the limit without it, 48 KB, holds for static and dynamic shared memory together

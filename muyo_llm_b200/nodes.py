@@ -128,8 +128,9 @@ def paged_cache_params(heads: int, kv_heads: int, head_dim: int, *, page_size: i
 
 
 def paged_plan_params(seqs: int, *, page_size: int, num_pages: int, table_stride: int,
-                      max_tokens: int) -> _abi.PagedPlanParams:
-    return _abi.PagedPlanParams(seqs, page_size, num_pages, table_stride, max_tokens)
+                      max_tokens: int, flags: int = 0) -> _abi.PagedPlanParams:
+    """flags: _abi.PLAN_ROOM admits requests that need no page behind one that found too few."""
+    return _abi.PagedPlanParams(seqs, page_size, num_pages, table_stride, max_tokens, flags)
 
 
 def paged_append_params(cache: _abi.PagedCache, tokens: int, *, n_dims: int | None = None, n_offs: int = 0,

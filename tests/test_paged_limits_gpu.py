@@ -105,6 +105,66 @@ def test_plan_of_rows_of_the_most_slots(cuda, page, width, pages, in_place):
     assert list(got) == list(want)
 
 
+def room_reference(cached, new, page, width, free, max_tokens):
+    """(lengths, refused, pages taken) where requests that need no page pass those that wait for some."""
+    lens, refused, taken, asked, total = [], 0, 0, 0, 0
+    for c, n in zip(cached, new):
+        total += max(n, 0)
+        fits = n > 0 and c + n <= width * page
+        need = -(-(c + n) // page) - -(-c // page) if fits else 0
+        asked += need
+        ok = fits and total <= max_tokens and (need == 0 or asked <= free)
+        taken += need if ok else 0
+        refused += n > 0 and not ok
+        lens.append(c + n if ok else 0 if n < 0 else c)
+    return lens, refused, taken
+
+
+@pytest.mark.parametrize("seqs,page,width,free,max_tokens,most", [
+    (2, 8, 4, 0, 2, 1), (60, 8, 20, 0, 200, 5), (300, 8, 20, 50, 9000, 30), (300, 8, 20, 50, 700, 30), (40, 1, 30, 9, 99, 4), (700, 16, 9, 0, 800, 2),
+])
+def test_plan_passes_requests_that_need_no_page(cuda, seqs, page, width, free, max_tokens, most):
+    """With MUYO_PLAN_ROOM a request that has room in its last page gets its tokens behind one that found no pages."""
+    rng = np.random.default_rng(seqs + free)
+    cached = [8, 3] if seqs == 2 else [int(rng.integers(0, page * width + 1)) for _ in range(seqs)]
+    new = [1, 1] if seqs == 2 else [int(rng.integers(-1, most + 1)) for _ in range(seqs)]
+    had = [-(-c // page) for c in cached]
+    ids = rng.permutation(sum(had) + free + 1).tolist()
+    table, at = [], 0
+    for h in had:
+        table.append(ids[at:at + h] + [-1] * (width - h))
+        at += h
+    head, pages = 11, len(ids)
+    ring = [-1] * pages
+    for k in range(free):
+        ring[(head + k) % pages] = ids[at + k]
+    lens, refused, taken = room_reference(cached, new, page, width, free, max_tokens)
+    p = nodes.paged_plan_params(seqs, page_size=page, num_pages=pages, table_stride=width, max_tokens=max_tokens, flags=_abi.PLAN_ROOM)
+    table_d, ring_d, lens_d, starts = ints(table), ints(ring), ints(cached), ints([0] * (seqs + 1))
+    positions, slots = ints([77] * max_tokens), ints([77] * max_tokens)
+    state = torch.tensor([head, head + free, 0, 0], device="cuda")
+    nodes.paged_plan(p, lens_d, ints(new), table_d, ring_d, state, lens_d, starts, positions, slots, state)
+    torch.cuda.synchronize()
+    back = sum(h for h, n in zip(had, new) if n < 0)
+    total = sum(max(n, 0) for n in new)
+    assert lens_d.tolist() == lens and state.tolist() == [head + taken, head + free + min(back, pages - free), refused, total]
+    if seqs == 2:
+        assert lens == [8, 4] and refused == 1
+    fresh = iter(ids[at:at + free])
+    slots, positions, table_d, t = slots.tolist(), positions.tolist(), table_d.tolist(), 0
+    for i, (c, n) in enumerate(zip(cached, new)):
+        row = table[i][:had[i]]
+        if lens[i] > c:
+            row += [next(fresh) for _ in range(-(-lens[i] // page) - had[i])]
+        assert table_d[i][:len(row)] == row and table_d[i][len(row):] == [-1] * (width - len(row))
+        for u in range(max(n, 0)):
+            if t < max_tokens:
+                pos = c + u if lens[i] > c else 0
+                assert (positions[t], slots[t]) == (pos, row[pos // page] * page + pos % page if lens[i] > c else -1), (i, t)
+            t += 1
+    assert all(s == -1 and x == 0 for s, x in zip(slots[t:], positions[t:]))
+
+
 # ---- attention ------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", [_abi.KV_F32, _abi.KV_F16, _abi.KV_F8])
