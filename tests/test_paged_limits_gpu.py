@@ -15,7 +15,7 @@ import torch
 
 from conftest import ROOT
 from muyo_llm_b200 import _abi, nodes
-from test_paged_gpu import DTYPES, Server, as_bits, attention64, gen, ints, plan_reference, randn, rotated64, run_plan
+from test_paged_gpu import DTYPES, as_bits, attention64, gen, ints, plan_reference, randn, rotated64, run_plan
 
 pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
@@ -210,3 +210,100 @@ def test_attention_of_scores_up_to_1e9(cuda, dtype, heads, kv, hd, sign):
         assert bool(((out[i].double() - want).abs() <= 16 * U * want.abs()).all()), (i, lens[i])
         score = sign * (q[i].double() * k[row].double().repeat_interleave(heads // kv, 0)).sum(-1)
         assert bool(((lse[i].double() - score).abs() <= (2 * hd + 20) * U * score.abs()).all()), (i, lse[i], score)
+
+
+# ---- a host's step ---------------------------------------------------------------------------------------------
+
+class Host:
+    """A decode step of several layers as a host makes it from the library's calls alone. The step's tokens are packed in
+    the requests' order. Each layer's q lies one row behind the start of its buffer, so that the row of request i's last
+    token is row query_start[i + 1] of the buffer (row 0 stands for no token); `owner`, which the host writes beside new_lens, brings the attention's
+    rows back to the tokens'. The layers are x + attention(x, x, x's first channels and its last ones)."""
+
+    def __init__(self, layers, seqs, heads, kv, hd, page, pages, width, stream):
+        self.stream, self.row, self.kv_row = stream, heads * hd, kv * hd
+        cache = nodes.paged_cache_params(heads, kv, hd, page_size=page, num_pages=pages, kv_dtype=_abi.KV_F32)
+        self.plan_p = nodes.paged_plan_params(seqs, page_size=page, num_pages=pages, table_stride=width, max_tokens=seqs, flags=_abi.PLAN_ROOM)
+        self.append_p = nodes.paged_append_params(cache, seqs, stride_k=self.row, stride_v=self.row)
+        self.attn_p = nodes.paged_attention_params(cache, seqs, table_stride=width)
+        self.gather_p, self.back_p = nodes.get_rows_params(self.row, seqs + 1, seqs), nodes.get_rows_params(self.row, seqs, seqs)
+        self.lens, self.new, self.owner, self.positions, self.slots = (ints([0] * seqs) for _ in range(5))
+        self.starts, self.ring = ints([0] * (seqs + 1)), ints(range(pages))
+        self.table = torch.full((seqs, width), -1, dtype=torch.int32, device="cuda")
+        self.state = torch.tensor([0, pages, 0, 0], device="cuda")
+        self.x, self.q_of, self.out, self.back = (torch.zeros((seqs, self.row), device="cuda") for _ in range(4))
+        self.y = torch.zeros((seqs, self.row), device="cuda")
+        self.q_rows = torch.zeros((seqs + 1, self.row), device="cuda")
+        self.pools = [[torch.full((pages, kv, page, hd), math.nan, device="cuda") for _ in range(2)] for _ in range(layers)]
+        self.freqs = torch.zeros(hd // 2 + 1, dtype=torch.float64, device="cuda")
+        nodes.rope_frequencies(nodes.rope_params(1, hd), self.freqs, stream=stream)
+        size = nodes.paged_attention_workspace_size(self.attn_p)
+        self.ws, self.ws_bytes = torch.empty(size, dtype=torch.uint8, device="cuda"), size
+
+    def step(self):
+        s = self.stream
+        nodes.paged_plan(self.plan_p, self.lens, self.new, self.table, self.ring, self.state, self.lens, self.starts,
+                         self.positions, self.slots, self.state, stream=s)
+        self.y.copy_(self.x)
+        for pools in self.pools:
+            nodes.paged_rope_append(self.append_p, self.y, self.y, self.y[:, self.row - self.kv_row:], self.positions, self.slots,
+                                    self.freqs, self.q_rows[1:], *pools, stream=s)
+            nodes.get_rows_f32(self.gather_p, self.q_rows, self.starts[1:], self.q_of, stream=s)
+            nodes.paged_attention_decode(self.attn_p, self.q_of, *pools, self.table, self.lens, self.out, self.ws, self.ws_bytes, stream=s)
+            nodes.get_rows_f32(self.back_p, self.out, self.owner, self.back, stream=s)
+            self.y.add_(self.back)
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_step_of_a_host(cuda, captured):
+    """Ended, idle and refused requests among the others, two layers: each token against its request's own cache in
+    64 bits. The first layer's error D (its tolerance, and the roundings of x + y) changes the second's scores by at
+    most scale hd D (max |q| + max |k|) and its values by D."""
+    layers, seqs, heads, kv, hd, page, pages, width = 2, 7, 8, 2, 64, 4, 22, 9
+    scale, row = 1.0 / math.sqrt(hd), heads * hd
+    g, rng, stream = gen(50), np.random.default_rng(51), torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        s = Host(layers, seqs, heads, kv, hd, page, pages, width, stream)
+        if captured:
+            s.step()  # nothing asked for: loads the modules
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                s.step()
+        empty = torch.zeros((0, kv, hd), dtype=torch.float64, device="cuda")
+        own = [[[empty, empty] for _ in range(layers)] for _ in range(seqs)]
+        length, answered, refused = [0] * seqs, 0, 0
+        for number in range(60):
+            new = [-1 if n and rng.random() < 0.04 else int(rng.random() < 0.8) for n in length]
+            owner = [i for i, n in enumerate(new) if n == 1]
+            s.new.copy_(ints(new))
+            s.owner.copy_(ints(owner + [-1] * (seqs - len(owner))))
+            s.x.copy_(randn(s.x.shape, g))
+            graph.replay() if captured else s.step()
+            stream.synchronize()
+            lens = s.lens.tolist()
+            for t, i in enumerate(owner):
+                if lens[i] == length[i]:
+                    refused += 1
+                    assert s.slots[t].item() == -1
+                    continue
+                x, D, pos = s.x[t].double().reshape(1, heads, hd), 0.0, s.positions[t:t + 1]
+                assert pos.item() == length[i] == lens[i] - 1
+                for k in range(layers):
+                    q = rotated64(x, pos, s.freqs, _abi.ROPE_NEOX, hd, 0)
+                    key, value = q[:, :kv], x[:, heads - kv:]
+                    own[i][k] = [torch.cat([own[i][k][0], key]), torch.cat([own[i][k][1], value])]
+                    out, _, tol, _ = attention64(q[0], *own[i][k], scale)
+                    most = [float(v.abs().max()) for v in (q, *own[i][k])]
+                    moved = scale * hd * (D + 2 * U * most[1]) * (most[0] + most[1])
+                    x = x + out
+                    D += float(tol.max()) + 4 * U * float(x.abs().max()) + 2 * moved * most[2] + D
+                assert float((s.y[t].double().reshape(heads, hd) - x[0]).abs().max()) <= D, (number, i)
+                length[i], answered = lens[i], answered + 1
+            for i, n in enumerate(new):
+                if n < 0:
+                    own[i], length[i] = [[empty, empty] for _ in range(layers)], 0
+                assert lens[i] == length[i], (number, i)
+        assert answered > 100 and refused > 3
+        if captured:
+            del graph
+    torch.cuda.synchronize()
