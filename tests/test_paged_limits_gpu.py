@@ -15,7 +15,7 @@ import torch
 
 from conftest import ROOT
 from muyo_llm_b200 import _abi, nodes
-from test_paged_gpu import DTYPES, as_bits, attention64, gen, ints, plan_reference, randn, rotated64, run_plan
+from test_paged_gpu import DTYPES, as_bits, attention64, gen, ints, plan_case, plan_reference, randn, rotated64, run_plan
 
 pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
@@ -307,3 +307,48 @@ def test_step_of_a_host(cuda, captured):
         if captured:
             del graph
     torch.cuda.synchronize()
+
+
+def test_step_is_repeated_after_a_refusal(cuda):
+    """In place: whoever got tokens asks for none in the repeated plan, one request ends, and a third plan serves the refused one from the pages
+    given back; no position is given twice and no page is lost."""
+    page, width, pages = 8, 6, 6
+    plan = nodes.paged_plan_params(4, page_size=page, num_pages=pages, table_stride=width, max_tokens=64)
+    lens, table, ring = ints([0] * 4), torch.full((4, width), -1, dtype=torch.int32, device="cuda"), ints(range(pages))
+    state, starts = torch.tensor([0, pages, 0, 0], device="cuda"), ints([0] * 5)
+    positions, slots = ints([0] * 64), ints([0] * 64)
+
+    def step(new):
+        nodes.paged_plan(plan, lens, ints(new), table, ring, state, lens, starts, positions, slots, state)
+        torch.cuda.synchronize()
+        first = starts.tolist()
+        return [a for a, n in enumerate(new) if n > 0 and slots[first[a]].item() == -1]  # the refused
+
+    assert step([10, 16, 30, 4]) == [2, 3] and lens.tolist() == [10, 16, 0, 0]
+    assert step([0, -1, 30, 4]) == [2, 3]  # the pages of ended requests serve the plans that follow
+    assert step([0, 0, 30, 4]) == [3] and lens.tolist() == [10, 0, 30, 0]
+    assert positions[:30].tolist() == list(range(30))
+    assert step([0, 0, 2, 0]) == [] and positions[:2].tolist() == [30, 31]
+    held = [x for i, n in enumerate(lens.tolist()) for x in table[i, :-(-n // page)].tolist()]
+    head, tail = state.tolist()[:2]
+    assert sorted(held + [ring[k % pages].item() for k in range(head, tail)]) == list(range(pages))
+
+
+def test_plan_apart_is_made_again_with_other_lengths(cuda):
+    """Outputs apart from the inputs: a plan that was not taken over leaves what the next one needs."""
+    args = plan_case(np.random.default_rng(8), 60, 8, 20, lambda r: r.integers(-1, 30), 40, 3)
+    cached, first, table, ring, state = args
+    second = [-1 if i % 7 == 3 else 0 if n > 20 else max(n, 0) for i, n in enumerate(first)]
+    p = nodes.paged_plan_params(60, page_size=8, num_pages=len(ring), table_stride=20, max_tokens=2000)
+    cached_d, table_d, ring_d = ints(cached), ints(table), ints(ring)
+    state_d, state_out = torch.tensor([*state, 0, 0], device="cuda"), torch.zeros(4, dtype=torch.int64, device="cuda")
+    lens, starts, positions, slots = ints([0] * 60), ints([0] * 61), ints([0] * 2000), ints([0] * 2000)
+    for new in (first, second):
+        nodes.paged_plan(p, cached_d, ints(new), table_d, ring_d, state_d, lens, starts, positions, slots, state_out)
+    torch.cuda.synchronize()
+    want = plan_reference(cached, second, table, ring, state, 8, 2000)
+    assert [lens.tolist(), starts.tolist(), positions.tolist(), slots.tolist(), state_out.tolist()] == list(want[2:])
+    for got, row, n in zip(table_d.tolist(), want[0], want[2]):
+        assert got[:-(-n // 8)] == row[:-(-n // 8)]
+    got = ring_d.tolist()
+    assert all(got[k % len(ring)] == want[1][k % len(ring)] for k in range(want[6][0], want[6][1]))
