@@ -11,10 +11,10 @@ from . import _abi
 
 
 def _ptr(t) -> int | None:
-    try:
-        return t.data_ptr()
-    except AttributeError:  # an address, or None
+    """Of a buffer or an address. Anything else raises: ctypes would pass bytes, text and arrays of the host on as they are."""
+    if t is None or isinstance(t, int):
         return t
+    return t.data_ptr()
 
 
 def _stream(s):
