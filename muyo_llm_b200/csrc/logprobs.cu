@@ -72,12 +72,21 @@ __device__ __forceinline__ unsigned long long warp_max_key(unsigned long long v)
     return (unsigned long long)most << 32 | lo;
 }
 
-// exp(u / T) 2^64: the sums are formed 2^64 times as large, so that terms down to 2^-190 of the largest stay normal.
+// exp(u / T) is 0 from 2^-126 on. Where that could be missed, 2^64 times as large: near u = 0 the added 64 would round the
+// exponent by 2^-18, so only where no weight is near 1, or where u is far.
 constexpr float kLogprobDown = 5.421010862427522e-20f;  // 2^-64
 __device__ __forceinline__ float weight_up(float u, float inv_t)
 {
     return ex2(fmaf(u, inv_t, 64.0f));
 }
+// a exp(u / T), also where exp(u / T) alone would be 0
+__device__ __forceinline__ float weighed(float a, float u, float inv_t)
+{
+    const float x = u * inv_t;
+    const bool far = x < -64.0f;
+    return a * ex2(far ? x + 64.0f : x) * (far ? kLogprobDown : 1.0f);
+}
+constexpr float kLogprobFew = 8.271806125530277e-25f;  // 2^-80
 constexpr float kLogprobLeast = -1.0e29f;  // u where the weight is 0, so that 0 * -inf does not arise
 
 // The ids below `end` from `begin` on at which x is `value`, in order, by one warp: lanes have .. top_k - 1 receive them
@@ -154,10 +163,10 @@ __device__ __forceinline__ LogprobPiece logprob_join_sums(const LogprobDev& p, L
         q = LogprobPiece{-INFINITY, 0.0f, 0.0f, 0};
     const float m = warp_max(q.m), ms = m == -INFINITY ? 0.0f : m;
     const bool top = here && q.m == m;
-    const float u = fmaxf(q.m - ms, kLogprobLeast), w = here ? weight_up(u, p.inv_t) : 0.0f;
+    const float u = fmaxf(q.m - ms, kLogprobLeast);
     LogprobPiece sum{m, 0.0f, 0.0f, 0};
-    sum.r = warp_sum(top ? q.r : (1.0f + q.r) * w * kLogprobDown) + (float)(__popc(__ballot_sync(0xffffffffu, top)) - 1);
-    sum.e = warp_sum(top ? q.e : fmaf(u, 1.0f + q.r, q.e) * w * kLogprobDown);
+    sum.r = warp_sum(top ? q.r : here ? weighed(1.0f + q.r, u, p.inv_t) : 0.0f) + (float)(__popc(__ballot_sync(0xffffffffu, top)) - 1);
+    sum.e = warp_sum(top ? q.e : here ? weighed(fmaf(u, 1.0f + q.r, q.e), u, p.inv_t) : 0.0f);
     sum.before = __reduce_add_sync(0xffffffffu, q.before);
     return sum;
 }
@@ -165,7 +174,8 @@ __device__ __forceinline__ LogprobPiece logprob_join_sums(const LogprobDev& p, L
 // One piece of a row: tiles of V float4 per thread, two tiles' loads under way, no barrier. A thread keeps its largest
 // logit so far, its sums of w and w (x - m) relative to it, and its count of ids in front of the token (looked
 // at where a tile's largest is not below the token's logit). Where little lies beside the largest, its 1 has
-// rounded the sum: then the sums are formed again without it, from a second read.
+// rounded the sum: then the sum is formed again without it, from a second read of its thread's logits; and where it is
+// below 2^-80, sums and moments from a second read of all, with weights that do not end at 2^-126.
 //
 // The first top_k ids: the threads' maxima, taken over 64 groups of 4 threads, give a threshold, the top_k-th
 // largest of them, that top_k logits reach and few others do (24 on average for 20 of 64). A warp
@@ -235,7 +245,7 @@ __global__ void __launch_bounds__(kLogprobThreads<TOP>, 1024 / kLogprobThreads<T
     // there is none: of a masked token, all ids below it are in front (added after the loop) and those above it that are
     // not masked. The four logits around the token have both kinds: put right after the loop.
     const float below = xt == -INFINITY ? INFINITY : nextafterf(xt, -INFINITY);
-    float m = -INFINITY, r = 0.0f, e = 0.0f;  // r, e: 2^64 times the sums
+    float m = -INFINITY, r = 0.0f, e = 0.0f;
     float front = 0.0f;  // ids in front of the token: exact, a thread has 1024 logits of a piece at most
     if (tid == 0)
         s_count = s_threads = 0;
@@ -245,12 +255,12 @@ __global__ void __launch_bounds__(kLogprobThreads<TOP>, 1024 / kLogprobThreads<T
         for (int j = 1; j < V; ++j)
             mine = fmaxf(fmaxf(mine, fmaxf(v[j].x, v[j].y)), fmaxf(v[j].z, v[j].w));
         const float mn = fmaxf(m, mine), ms = mn == -INFINITY ? 0.0f : mn;
-        const float2 scale = make_float2(p.inv_t, p.inv_t), up = make_float2(64.0f, 64.0f), back = make_float2(-ms, -ms);
-        float2 sum = make_float2(0.0f, 0.0f), moment = sum;
+        const float2 scale = make_float2(p.inv_t, p.inv_t), back = make_float2(-ms, -ms), zero = make_float2(0.0f, 0.0f);
+        float2 sum = zero, moment = zero;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const float2 u0 = add2(make_float2(v[j].x, v[j].y), back), u1 = add2(make_float2(v[j].z, v[j].w), back);
-            const float2 x0 = fma2(u0, scale, up), x1 = fma2(u1, scale, up);  // as in weight_up
+            const float2 x0 = fma2(u0, scale, zero), x1 = fma2(u1, scale, zero);
             const float2 w0 = make_float2(ex2(x0.x), ex2(x0.y)), w1 = make_float2(ex2(x1.x), ex2(x1.y));
             sum = add2(sum, add2(w0, w1));
             moment = fma2(w0, make_float2(fmaxf(u0.x, kLogprobLeast), fmaxf(u0.y, kLogprobLeast)), moment);
@@ -258,7 +268,7 @@ __global__ void __launch_bounds__(kLogprobThreads<TOP>, 1024 / kLogprobThreads<T
         }
         const float tr = sum.x + sum.y, te = moment.x + moment.y;
         // the sums so far, relative to the new largest (at 0 before the first logit above -inf)
-        const float u = fmaxf(m - ms, kLogprobLeast), w = weight_up(u, p.inv_t) * kLogprobDown;
+        const float u = fmaxf(m - ms, kLogprobLeast), w = ex2(u * p.inv_t);
         e = w > 0.0f ? fmaf(w, fmaf(u, r, e), te) : te;  // u * r is finite where w is not 0
         r = fmaf(w, r, tr);
         m = mn;
@@ -308,7 +318,7 @@ __global__ void __launch_bounds__(kLogprobThreads<TOP>, 1024 / kLogprobThreads<T
     for (int w = 0; w < WARPS; ++w)
         M = fmaxf(M, s_m[w]);
     {
-        const float u = fmaxf(m - (M == -INFINITY ? 0.0f : M), kLogprobLeast), w = weight_up(u, p.inv_t) * kLogprobDown;
+        const float u = fmaxf(m - (M == -INFINITY ? 0.0f : M), kLogprobLeast), w = ex2(u * p.inv_t);
         e = w > 0.0f ? fmaf(u, r, e) * w : 0.0f;
         r *= w;
     }
@@ -342,36 +352,62 @@ __global__ void __launch_bounds__(kLogprobThreads<TOP>, 1024 / kLogprobThreads<T
 #pragma unroll
     for (int w = 0; w < WARPS; ++w)
         sum.r += s_r[w], sum.e += s_e[w], sum.before += s_before[w];
-    sum.r *= kLogprobDown;
-    sum.e *= kLogprobDown;
     if (M == -INFINITY) {
         sum.r = sum.r == sum.r ? 0.0f : NAN;
         sum.e = 0.0f;
     } else if (sum.r < 1.25f) {
         // one logit is the largest, or the sum would be 2 or more: its thread's logits again, a float4 per lane
         const unsigned holder = __ballot_sync(0xffffffffu, m == M);
+        float next = m == M ? -INFINITY : m;  // the largest of the others
         __syncthreads();
         if (holder) {
             const int from = __ffs(holder) - 1, i0 = origin + (warp * 32 + from) * 4;
             float rest = lane == from ? 0.0f : own;
+            const auto add = [&](float y) {
+                rest += y == M ? 0.0f : ex2((y - M) * p.inv_t);
+                next = fmaxf(next, y == M ? -INFINITY : y);
+            };
 #pragma unroll 1
             for (int q = lane; q < V * tiles; q += 32) {
                 const float4 f = quad(i0 + q / V * TILE + q % V * Q);
-                rest += f.x == M ? 0.0f : weight_up(f.x - M, p.inv_t);
-                rest += f.y == M ? 0.0f : weight_up(f.y - M, p.inv_t);
-                rest += f.z == M ? 0.0f : weight_up(f.z - M, p.inv_t);
-                rest += f.w == M ? 0.0f : weight_up(f.w - M, p.inv_t);
+                add(f.x), add(f.y), add(f.z), add(f.w);
             }
             rest = warp_sum(rest);
             if (lane == 0)
                 s_r[warp] = rest;
         }
-        __syncthreads();
+        const bool more = __syncthreads_or(weight_up(next - M, p.inv_t) > 0.0f);
         sum.r = 0.0f;
 #pragma unroll
         for (int w = 0; w < WARPS; ++w)
             sum.r += s_r[w];
-        sum.r *= kLogprobDown;
+        if (sum.r < kLogprobFew && more) {
+            // The others' weights are all far below 1, and some have come out as 0 (less than 2^-107 together, which a
+            // larger sum does not miss): every thread's logits again.
+            r = e = 0.0f;
+            const auto add = [&](float y) {
+                const float u = y == M ? -INFINITY : y - M, w = weight_up(u, p.inv_t);
+                r += w;
+                e = fmaf(w, fmaxf(u, kLogprobLeast), e);
+            };
+#pragma unroll 1
+            for (int q = 0; q < V * tiles; ++q) {
+                const float4 f = quad(origin + q / V * TILE + q % V * Q + tid * 4);
+                add(f.x), add(f.y), add(f.z), add(f.w);
+            }
+            r = warp_sum(r);
+            e = warp_sum(e);
+            __syncthreads();  // s_r is read
+            if (lane == 0)
+                s_r[warp] = r, s_e[warp] = e;
+            __syncthreads();
+            sum.r = sum.e = 0.0f;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w)
+                sum.r += s_r[w], sum.e += s_e[w];
+            sum.r *= kLogprobDown;
+            sum.e *= kLogprobDown;
+        }
     } else {
         sum.r -= 1.0f;
     }
@@ -553,10 +589,10 @@ __global__ void __launch_bounds__(kLogprobJoinThreads) k_logprob_join(LogprobDev
     for (int c = tid; c < p.pieces; c += kLogprobJoinThreads) {
         const LogprobPiece q = mine[c];
         const bool top = q.m == m;
-        const float u = fmaxf(q.m - ms, kLogprobLeast), w = weight_up(u, p.inv_t);
-        r += top ? q.r : (1.0f + q.r) * w * kLogprobDown;
+        const float u = fmaxf(q.m - ms, kLogprobLeast);
+        r += top ? q.r : weighed(1.0f + q.r, u, p.inv_t);
         equal += top;
-        e += top ? q.e : fmaf(u, 1.0f + q.r, q.e) * w * kLogprobDown;
+        e += top ? q.e : weighed(fmaf(u, 1.0f + q.r, q.e), u, p.inv_t);
         before += q.before;
     }
     r = warp_sum(r);

@@ -1,0 +1,81 @@
+"""Log probabilities where single weights show, where sums are far below 1, and where rows are cut in every way.
+
+U = 2^-24. A weight w = exp(d), d = (x - m) / T, is off by at most (3 |d| + 8) U of itself: the difference, the scaling's
+two roundings, and the exponential (2^-22, or 4 U)."""
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from test_token_logprobs_gpu import gen, score
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+@pytest.mark.parametrize("vocab", [2, 40, 5000, 151936])
+@pytest.mark.parametrize("temperature", [1.0, 0.7, 30.0])
+def test_single_weights(cuda, vocab, temperature):
+    """Two tokens and masked ones: log p of the larger is -log(1 + w), of the smaller d - log(1 + w), with one weight w. log(1 + w) is off by the
+    weight's error, w (3 |d| + 8) U, and by the 3 U of its logarithm and of the rounding of 1 + w's argument."""
+    T = float(np.float32(temperature))
+    gaps = torch.cat([torch.linspace(0.01, 6.0, 500), torch.linspace(6.0, 80.0, 50), torch.linspace(80.0, 86.0, 5)])
+    gaps = ((gaps.double() * T).float()).cuda()
+    if vocab > 5000:
+        gaps = gaps[::9].contiguous()
+    rows = len(gaps)
+    logits = torch.full((rows, vocab), -math.inf, device="cuda")
+    at = torch.randint(0, vocab, (rows,), generator=gen(vocab), device="cuda")
+    to = (at + 1 + torch.randint(0, vocab - 1, (rows,), generator=gen(vocab + 1), device="cuda")) % vocab
+    row = torch.arange(rows, device="cuda")
+    logits[row, at] = 0.0
+    logits[row, to] = -gaps
+    d = -gaps.double() / T
+    w = torch.exp(d)
+    norm = torch.log1p(w)
+    tol = w / (1 + w) * (3 * d.abs() + 8) * U + 3 * U * norm
+    for tokens, want, more in ((at, -norm, 0.0), (to, d - norm, 4 * U * d.abs())):
+        for top in (0, 2):
+            lp, h, rank, ids, tops = score(logits, tokens.to(torch.int32), top, temperature)
+            err = (lp.double() - want).abs()
+            assert bool((err <= tol + more).all()), ((err / (tol + more)).max().item(), gaps[int((err / (tol + more)).argmax())].item())
+            entropy = norm - d * w / (1 + w)
+            tol_h = (w / (1 + w) * (d.abs() + 1) * (3 * d.abs() + 16)) * U + 4 * U * entropy
+            assert bool(((h.double() - entropy).abs() <= tol_h).all())
+            if top:
+                assert bool(((tops[:, 0].double() + norm).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("rows", [1, 30, 700])
+@pytest.mark.parametrize("fill", [-math.inf, torch.finfo(torch.float32).min])
+def test_sums_far_below_one(cuda, rows, fill):
+    """1 + R with R from 1e-35 to 1e-10, of many equal weights or of a few in the largest's own thread, piece and
+    elsewhere: R keeps its relative accuracy. |d| is below 90, the sum adds 128 U."""
+    vocab = 32003
+    logits = torch.full((rows, vocab), fill, device="cuda")
+    best = torch.randint(0, vocab, (rows,), generator=gen(rows), device="cuda")
+    gap = torch.linspace(25.0, 80.0, rows, device="cuda")
+    kind = torch.arange(rows, device="cuda") % 3
+    for i in range(rows):
+        b, lo = int(best[i]), -float(gap[i])
+        if kind[i] == 0:
+            logits[i] = lo
+        elif kind[i] == 1:  # neighbours share a thread
+            logits[i, max(b - 3, 0):b + 4] = lo
+        else:
+            logits[i, (b + 17000) % vocab] = lo
+        logits[i, b] = 0.0
+    d = logits.double()
+    w = torch.exp(d)
+    w[torch.arange(rows, device="cuda"), best] = 0.0
+    R = w.sum(1)
+    weighed = (w * d.clamp(min=-1e4)).sum(1)
+    for top in (0, 5):
+        lp, h, _, _, _ = score(logits, best.to(torch.int32), top)
+        want = -torch.log1p(R)
+        assert bool(((lp.double() - want).abs() <= 410 * U * want.abs()).all()), ((lp.double() - want) / want).abs().max().item()
+        entropy = torch.log1p(R) - weighed / (1 + R)
+        assert bool(((h.double() - entropy).abs() <= 800 * U * entropy).all())
