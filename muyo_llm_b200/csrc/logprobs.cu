@@ -122,7 +122,11 @@ struct LogprobRow {
     }
     __device__ __forceinline__ float log_p(float x) const
     {
-        return nothing ? -INFINITY : __fdiv_rn(x - m, temperature) - log_sum;
+        if (nothing)
+            return -INFINITY;
+        const float d = x - m;
+        // two finite logits may lie further apart than F32 reaches, and their difference by the temperature does not
+        return (d == -INFINITY ? 2.0f * __fdiv_rn(0.5f * x - 0.5f * m, temperature) : __fdiv_rn(d, temperature)) - log_sum;
     }
     __device__ __forceinline__ void write(const LogprobDev& p, const LogprobOut& out, const LogprobPiece& q, int row, int token,
                                           float xt) const

@@ -79,3 +79,20 @@ def test_sums_far_below_one(cuda, rows, fill):
         assert bool(((lp.double() - want).abs() <= 410 * U * want.abs()).all()), ((lp.double() - want) / want).abs().max().item()
         entropy = torch.log1p(R) - weighed / (1 + R)
         assert bool(((h.double() - entropy).abs() <= 800 * U * entropy).all())
+
+
+def test_differences_beyond_f32(cuda):
+    """Finite logits whose difference is not: log p is finite where (x - m) / T is, within 4 U of it."""
+    big = torch.finfo(torch.float32).max
+    logits = torch.full((2, 100), -math.inf, device="cuda")
+    logits[:, 7], logits[:, 8], logits[:, 50] = big, -big, 0.0
+    for temperature in (1e6, 3.0, 1.0):
+        lp, h, rank, ids, tops = score(logits, torch.tensor([8, 7], dtype=torch.int32, device="cuda"), 4, temperature)
+        T = float(np.float32(temperature))
+        want = -2.0 * big / T
+        if abs(want) < big:
+            assert abs(float(lp[0]) - want) <= 4 * U * abs(want) and abs(float(tops[0, 2]) - want) <= 4 * U * abs(want)
+        else:
+            assert float(lp[0]) == -math.inf and float(tops[0, 2]) == -math.inf
+        assert float(lp[1]) == 0.0 and float(h[0]) == 0.0
+        assert rank.tolist() == [2, 0] and ids[0].tolist() == [7, 50, 8, 0] and float(tops[0, 3]) == -math.inf
