@@ -556,7 +556,7 @@ typedef struct MuyoPagedAttentionParams {
     uint32_t table_stride; /* pages of a table row; table_stride * page_size at most 2^30 */
     uint32_t window;
     uint32_t stride_q, stride_out; /* 0 = packed rows */
-    float scale;
+    float scale;           /* |scale| and |scale * k_scale| at most 2^127 */
 } MuyoPagedAttentionParams;
 size_t muyo_cuda_paged_attention_workspace_size(const MuyoPagedAttentionParams* p);
 int muyo_cuda_paged_attention_decode(const MuyoPagedAttentionParams* p, const float* q, const void* k_pool,

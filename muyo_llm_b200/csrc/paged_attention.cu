@@ -1013,7 +1013,9 @@ static int paged_attention_prepare(const MuyoPagedAttentionParams* p, PagedAttnD
     MUYO_REQUIRE(p->table_stride > 0 && (uint64_t)p->cache.page_size * p->table_stride <= (uint64_t)1 << 30,
                  "paged_attention: table_stride %u must be positive, and a row at most 2^30 slots", p->table_stride);
     MUYO_REQUIRE(p->window <= (uint32_t)INT_MAX, "paged_attention: window %u exceeds INT32_MAX", p->window);
-    MUYO_REQUIRE(std::isfinite(p->scale), "paged_attention: scale must be finite");
+    // scores are formed in powers of two
+    MUYO_REQUIRE(std::isfinite(p->scale * d.c.k_scale * 1.4426950408889634f),
+                 "paged_attention: scale and scale * k_scale must be at most 2^127");
     const uint32_t row = p->cache.heads * p->cache.head_dim;
     d.stride_q = p->stride_q ? p->stride_q : row;
     d.stride_out = p->stride_out ? p->stride_out : row;

@@ -12,3 +12,11 @@ from test_paged_cpu import EINVAL, EUNSUPPORTED, A, cache, lib, refused  # noqa:
 def test_plan_refuses_unknown_flags(lib):  # noqa: F811
     p = nodes.paged_plan_params(4, page_size=16, num_pages=64, table_stride=8, max_tokens=32, flags=2)
     refused(EINVAL, "muyo_cuda_paged_plan", p, *[A] * 10, None, match="flags")
+
+
+@pytest.mark.parametrize("scale,k_scale", [(1e30, 2.0 ** 100), (-3e38, 2.0), (3e38, 1.0)])
+def test_attention_refuses_scales_whose_product_overflows(lib, scale, k_scale):  # noqa: F811
+    """Each is in its range, but scores are scaled by both (and by log2 e): an infinite factor would give NaN."""
+    p = nodes.paged_attention_params(cache(kv_dtype=_abi.KV_F8, k_scale=k_scale), 4, table_stride=8, scale=scale)
+    refused(EINVAL, "muyo_cuda_paged_attention_decode", p, A, A, A, A, A, A, None, A, 1 << 30, None, match="scale")
+    assert lib.muyo_cuda_paged_attention_workspace_size(C.byref(p)) == 0
