@@ -1021,10 +1021,10 @@ static int paged_attention_prepare(const MuyoPagedAttentionParams* p, PagedAttnD
     d.stride_out = p->stride_out ? p->stride_out : row;
     MUYO_REQUIRE(d.stride_q >= row && d.stride_out >= row, "paged_attention: a row stride is below the row of %u", row);
     MUYO_REQUIRE((d.stride_q | d.stride_out) % 4 == 0, "paged_attention: row strides must be multiples of 4");
-    // tiles hold 8 keys or more
+    // tiles hold 8 keys or more; the kernel rounds their number up to whole CTAs
     const uint64_t tiles = ((uint64_t)p->cache.page_size * p->table_stride / 8 + 1) * p->cache.kv_heads;
-    if (tiles > (uint64_t)INT_MAX / p->seqs) {
-        set_error("paged_attention: %u requests of rows of %u pages are more than 2^31 tiles", p->seqs, p->table_stride);
+    if (tiles > (uint64_t)(INT_MAX - kPagedWarps) / p->seqs) {
+        set_error("paged_attention: %u requests of rows of %u pages are more than 2^31 - 5 tiles", p->seqs, p->table_stride);
         return MUYO_EUNSUPPORTED;
     }
     d.seqs = (int)p->seqs, d.table_stride = (int)p->table_stride, d.window = (int)p->window;

@@ -20,3 +20,11 @@ def test_attention_refuses_scales_whose_product_overflows(lib, scale, k_scale): 
     p = nodes.paged_attention_params(cache(kv_dtype=_abi.KV_F8, k_scale=k_scale), 4, table_stride=8, scale=scale)
     refused(EINVAL, "muyo_cuda_paged_attention_decode", p, A, A, A, A, A, A, None, A, 1 << 30, None, match="scale")
     assert lib.muyo_cuda_paged_attention_workspace_size(C.byref(p)) == 0
+
+
+@pytest.mark.parametrize("heads,page,width,seqs", [(1, 25, 38177487, 18), (1, 1 << 20, 1 << 10, 16)])
+def test_attention_refuses_more_tiles_than_a_count_holds(lib, heads, page, width, seqs):  # noqa: F811
+    """2^31 - 2 tiles fit the count, but not what is added to it to round up to whole CTAs."""
+    p = nodes.paged_attention_params(cache(heads=heads, kv_heads=1, page_size=page, num_pages=4), seqs, table_stride=width)
+    refused(EUNSUPPORTED, "muyo_cuda_paged_attention_decode", p, A, A, A, A, A, A, None, A, 1 << 30, None, match="tiles")
+    assert lib.muyo_cuda_paged_attention_workspace_size(C.byref(p)) == 0
