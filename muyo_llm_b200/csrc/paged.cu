@@ -326,7 +326,7 @@ constexpr int kAppendThreads = 128;
 template <typename KV, bool V4>
 __global__ void __launch_bounds__(kAppendThreads, 8) k_paged_append(AppendDev p, const float* q, const float* k, const float* v,
                                                                  const int32_t* positions, const int32_t* slots,
-                                                                 const double* __restrict__ freqs, float* q_out, KV* k_pool,
+                                                                 const double* freqs, float* q_out, KV* k_pool,
                                                                  KV* v_pool)
 {
     __shared__ __align__(16) double cs[128];  // cos of pair j, then sin

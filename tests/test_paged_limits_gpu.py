@@ -352,3 +352,39 @@ def test_plan_apart_is_made_again_with_other_lengths(cuda):
         assert got[:-(-n // 8)] == row[:-(-n // 8)]
     got = ring_d.tolist()
     assert all(got[k % len(ring)] == want[1][k % len(ring)] for k in range(want[6][0], want[6][1]))
+
+
+def test_append_reads_a_table_made_before_it(cuda):
+    """Two tables by turns into one buffer, between appends of one captured graph."""
+    tokens, hd = 40, 64
+    g, stream = gen(60), torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        x = randn((tokens, hd), g)
+        positions, slots = ints(range(100, 100 + tokens)), ints(range(tokens))
+        cache = nodes.paged_cache_params(1, 1, hd, page_size=tokens, num_pages=1, kv_dtype=_abi.KV_F32)
+        freqs = torch.zeros(hd // 2 + 1, dtype=torch.float64, device="cuda")
+        pools = [torch.zeros((tokens, hd), device="cuda") for _ in range(5)]
+        bases = [10000.0, 500000.0, 30.0, 1e6]
+
+        def run():
+            for base, pool in zip(bases, pools):
+                nodes.rope_frequencies(nodes.rope_params(1, hd, freq_base=base), freqs, stream=stream)
+                nodes.paged_rope_append(nodes.paged_append_params(cache, tokens), None, x, x, positions, slots, freqs, None, pool, pools[4],
+                                        stream=stream)
+
+        run()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            run()
+        for _ in range(20):
+            x.copy_(randn(x.shape, g))
+            graph.replay()
+            stream.synchronize()
+            for base, pool in zip(bases, pools):
+                j = torch.arange(hd // 2, dtype=torch.float64, device="cuda")
+                table = torch.cat([base ** (-2.0 * j / hd), torch.ones(1, dtype=torch.float64, device="cuda")])
+                want = rotated64(x.double().reshape(tokens, 1, hd), positions, table, _abi.ROPE_NEOX, hd, 0)[:, 0]
+                # one rounding, and angles of at most 140 off by 2^-45
+                assert bool(((pool.double() - want).abs() <= U * want.abs() + 1e-11).all()), base
+        del graph
+    torch.cuda.synchronize()
