@@ -89,6 +89,18 @@ __device__ __forceinline__ float weighed(float a, float u, float inv_t)
 constexpr float kLogprobFew = 8.271806125530277e-25f;  // 2^-80
 constexpr float kLogprobLeast = -1.0e29f;  // u where the weight is 0, so that 0 * -inf does not arise
 
+// Four logits, which are read once: no L1 allocation. Not by the read-only path: an earlier kernel of the stream, whose
+// end this one waits for, may have written them after this one began.
+__device__ __forceinline__ float4 ld_logits(const float* p)
+{
+    float4 r;
+    asm volatile("ld.global.L1::no_allocate.v4.f32 {%0,%1,%2,%3}, [%4];"
+                 : "=f"(r.x), "=f"(r.y), "=f"(r.z), "=f"(r.w)
+                 : "l"(p)
+                 : "memory");
+    return r;
+}
+
 // The ids below `end` from `begin` on at which x is `value`, in order, by one warp: lanes have .. top_k - 1 receive them
 // (-1 without one).
 __device__ __forceinline__ int logprob_equal_ids(const float* x, float value, int begin, int end, int have, int top_k)
@@ -217,7 +229,7 @@ __global__ void __launch_bounds__(kLogprobThreads<TOP>, 1024 / kLogprobThreads<T
     const int tiles = (end - origin + TILE - 1) / TILE;
     const auto quad = [&](int i) {
         if (i >= 0 && i <= p.vocab - 4)
-            return ld_stream16f(x + i);
+            return ld_logits(x + i);
         float4 f = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
@@ -231,7 +243,7 @@ __global__ void __launch_bounds__(kLogprobThreads<TOP>, 1024 / kLogprobThreads<T
         if (i - tid * 4 >= 0 && i - tid * 4 + TILE <= p.vocab) {
 #pragma unroll
             for (int j = 0; j < V; ++j)
-                v[j] = ld_stream16f(x + i + j * Q);
+                v[j] = ld_logits(x + i + j * Q);
         } else {
 #pragma unroll 1
             for (int j = 0; j < V; ++j) {

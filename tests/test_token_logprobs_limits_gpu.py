@@ -10,6 +10,7 @@ import numpy as np
 import pytest
 import torch
 
+from muyo_llm_b200 import nodes
 from test_token_logprobs_gpu import gen, score
 
 pytestmark = pytest.mark.gpu
@@ -96,3 +97,40 @@ def test_differences_beyond_f32(cuda):
             assert float(lp[0]) == -math.inf and float(tops[0, 2]) == -math.inf
         assert float(lp[1]) == 0.0 and float(h[0]) == 0.0
         assert rank.tolist() == [2, 0] and ids[0].tolist() == [7, 50, 8, 0] and float(tops[0, 3]) == -math.inf
+
+
+def test_logits_of_the_kernel_before(cuda):
+    """Logits written by a kernel of the library right in front, replayed with new ones."""
+    rows, vocab = 64, 4001
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        a, b = (torch.zeros((rows, vocab), device="cuda") for _ in range(2))
+        logits = torch.zeros((rows, vocab), device="cuda")
+        tokens = torch.randint(0, vocab, (rows,), generator=gen(70), device="cuda").to(torch.int32)
+        lp, rank = torch.zeros(rows, device="cuda"), torch.zeros(rows, dtype=torch.int32, device="cuda")
+        p = nodes.token_logprobs_params(rows, vocab)
+        size = nodes.token_logprobs_workspace_size(p)
+        ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+
+        def step():
+            nodes.add(nodes.add_params(rows * vocab), a, b, logits, stream=stream)
+            nodes.token_logprobs(p, logits, tokens, lp, ws, size, rank=rank, stream=stream)
+
+        step()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            for _ in range(3):
+                step()
+        for seed in range(20):
+            a.copy_(torch.randn(a.shape, generator=gen(seed), device="cuda") * 3)
+            b.copy_(torch.randn(b.shape, generator=gen(seed + 100), device="cuda"))
+            graph.replay()
+            stream.synchronize()
+            x = a + b
+            given = x.gather(1, tokens.long()[:, None])
+            assert torch.equal(rank.long(), (x > given).sum(1) + ((x == given) & (torch.arange(vocab, device="cuda")[None] < tokens[:, None])).sum(1))
+            want = torch.log_softmax(x.double(), 1).gather(1, tokens.long()[:, None])[:, 0]
+            # the largest weights' d is below 40: 136 + 3 * 40 roundings, and 3 of d
+            assert bool(((lp.double() - want).abs() <= 400 * U).all())
+        del graph
+    torch.cuda.synchronize()
