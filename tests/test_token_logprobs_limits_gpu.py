@@ -134,3 +134,45 @@ def test_logits_of_the_kernel_before(cuda):
             assert bool(((lp.double() - want).abs() <= 400 * U).all())
         del graph
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("rows", [4, 40, 200, 900])
+@pytest.mark.parametrize("vocab,top_k", [(60000, 32), (60001, 20), (8190, 32)])
+def test_overfull_lists_in_rows_of_every_cut(cuda, rows, vocab, top_k):
+    """Rising rows, steps of whole tiles, repeated ramps, constant rows, the lowest value, a few values: more logits reach the
+    threshold than are listed, in rows of one piece, of a cluster and of many pieces."""
+    index = torch.arange(vocab, device="cuda")
+    lowest = torch.full((vocab,), torch.finfo(torch.float32).min, device="cuda")
+    kinds = [index * 1e-3, (index // 4096).float(), (index % 1024).float() * 0.01, torch.full((vocab,), 2.5, device="cuda"), lowest,
+             -(index // 600).float(), torch.round(torch.randn(vocab, generator=gen(vocab), device="cuda")),
+             torch.where(index % 13 == 5, 1.0, lowest), torch.where(index % 2 == 0, index * 1e-4, -math.inf)]
+    base = torch.stack(kinds)
+    kind = torch.arange(rows, device="cuda") % len(kinds)
+    logits = base[kind].contiguous()
+    tokens = torch.randint(0, vocab, (rows,), generator=gen(rows), device="cuda")
+    lp, h, rank, ids, tops = score(logits, tokens.to(torch.int32), top_k)
+    d = (base.double() - base.double().amax(1, keepdim=True))
+    w = torch.exp(d)
+    best = base.argmax(1, keepdim=True)
+    w = w.scatter(1, best, 0.0)
+    R = w.sum(1, keepdim=True)
+    norm, p = torch.log1p(R), w / (1 + R)
+    finite = d.clamp(min=-1e4).abs()
+    tol = U * (p * (3 * finite + 136)).sum(1, keepdim=True) + 2 * U * norm
+    order = torch.sort(base, dim=1, descending=True, stable=True).indices[:, :top_k]
+    place = torch.empty_like(base, dtype=torch.int64)
+    place.scatter_(1, torch.sort(base, dim=1, descending=True, stable=True).indices, index.expand_as(place))
+    assert torch.equal(ids.long(), order[kind])
+    assert torch.equal(rank.long(), place[kind, tokens])
+
+    def near(got, at_kind, at_id):
+        dd = d[at_kind, at_id]
+        want = dd - norm[at_kind, 0]
+        return bool(((got.double() == want) | ((got.double() - want).abs() <= tol[at_kind, 0] + 3 * U * dd.abs() + U * want.abs())).all())
+
+    assert near(lp, kind, tokens)
+    for k in range(top_k):
+        assert near(tops[:, k], kind, ids[:, k].long())
+    entropy = (norm + (p * finite).sum(1, keepdim=True))[:, 0]
+    tol_h = U * (p * (finite + 1) * (3 * finite + 300)).sum(1) + 2 * U * entropy
+    assert bool(((h.double() - entropy[kind]).abs() <= tol_h[kind]).all())
