@@ -575,7 +575,8 @@ int muyo_cuda_paged_attention_decode(const MuyoPagedAttentionParams* p, const fl
  * The sum over the other tokens is kept apart from the largest's 1, so that log p of an almost certain
  * token keeps its relative accuracy. -inf logits (masked ids) have log p -inf; a row of nothing else
  * has log p -inf, entropy 0 and ids 0 .. top_k - 1. A row with a NaN or +inf gives NaN log
- * probabilities and entropy; NaN logits do not enter top_ids, and places that no id is left for hold -1.
+ * probabilities and entropy (its rank is not specified); NaN logits do not enter top_ids, and places that no id is left
+ * for hold -1. A row with fewer than top_k logits that are not NaN takes milliseconds.
  * logits are 4-byte aligned, in any stride; pointers are of the current device. One call at a time may use a
  * workspace; it may hold anything before. */
 typedef struct MuyoTokenLogprobsParams {

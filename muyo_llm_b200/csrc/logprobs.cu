@@ -202,9 +202,14 @@ __device__ __forceinline__ LogprobPiece logprob_join_sums(const LogprobDev& p, L
 //
 // Bound by the read, 4 bytes a logit: 2001 rows of 32001, 256 MB, take 51 us (5.0 TB/s, 0.76 of the copy rate; a CTA's
 // first loads and its last sums are a third of its time, the count for the rank 2 us and the entropy's sum 3 us of the
-// call), 97 rows of 151936 with 20 alternatives, 59 MB, 23.2 us (the
-// loop ends at 40% of the kernel's time, the rest is the second reads and the cluster's join), one row 8.5 us. Listing
+// call), 97 rows of 151936 with 20 alternatives, 59 MB, 23.0 us (the
+// loop ends at 40% of the kernel's time, the rest is the second reads and the cluster's join), one row 8.8 us. Listing
 // tile by tile in the loop took 40 us for the 97 rows, whole pieces in shared memory 59 us.
+//
+// Slower contents, all exact: more than 512 logits of a piece above the threshold (whole tiles that rise by steps) take
+// top_k passes over the piece, 97 rows 0.55 ms and 2001 rows 2.2 ms; constant rows 0.1 and 0.4 ms; a row with
+// fewer than top_k logits that are not NaN is searched for masked ones by one warp, 1.5 ms for a row of 151936 and 2.5 ms for
+// 97. Rows of almost certain tokens (the others' sum below 2^-80) take 2 to 4 us more.
 template <bool TOP, int V>
 __global__ void __launch_bounds__(kLogprobThreads<TOP>, 1024 / kLogprobThreads<TOP>)
                                                       k_logprob_pieces(LogprobDev p, const float* logits,

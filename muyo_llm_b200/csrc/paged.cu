@@ -17,8 +17,9 @@ namespace muyo {
 // finds its request by a binary search in the sums: all outputs are written in parallel from shared
 // memory, whatever the mix of long prompts and single tokens. A cluster of 8 CTAs shares that work; each forms
 // the sums for itself, and nothing is written before all have read what a step in place overwrites. Latency bound
-// (the sums, a binary search and a page look-up per token): 1501 requests with 48000 new tokens take 12 us, with one CTA
-// and divisions for pages and ring places 69 us; 250 single tokens 5 us, which is the call's own cost.
+// (the sums, a binary search and a page look-up per token): 1501 requests with 48000 new tokens take 12.1 us, with one CTA
+// and divisions for pages and ring places 69 us; 250 single tokens 4.9 to 5.6 us, which is the call's own cost.
+// Not separated by measurement: the sums, which every CTA forms in full, the barrier, and the tokens' searches.
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanCtas = 8;
 constexpr int kPlanMaxSeqs = 8192;
@@ -275,7 +276,7 @@ __device__ __forceinline__ void pool_store4<__nv_fp8_e4m3>(__nv_fp8_e4m3* dst, f
 
 // x / scale rounded to F32. For F16 and e4m3 pools as a product in float64 with the scale's reciprocal, which gives the
 // same F32: a quotient of two F32 that is not on a border between F32 values is 2^-49 of itself or more away from it, and the
-// product is off by 2^-52 at most. The division takes 5% more (6001 tokens into an e4m3 pool: 43.4 us, by division 45.5 us).
+// product is off by 2^-52 at most. The division takes 4% more (6001 tokens into an e4m3 pool, timed in turn).
 struct PoolScale {
     float scale;
     double inverse;
@@ -316,8 +317,8 @@ __device__ __forceinline__ void turn(float& a, float& b, double c, double s)
 // heads. V4: a thread's unit is two float4 of a row - four pairs, or eight channels that pass unchanged, or eight
 // channels of v, the second float4 half a range behind the first so that neighbours' accesses join up - all loaded
 // before the angles are waited for; else a unit is one pair. Bound by the bytes
-// (q twice, k and v once, the pools' rows): 6001 tokens of 32/8 heads of 128 into an e4m3 pool, 259 MB, take 43.4 us (6.0
-// TB/s, 0.91 of the copy rate); the float64 rotation costs 2 us of it. Eight CTAs of four warps on an SM keep loads, turns and
+// (q twice, k and v once, the pools' rows): 6001 tokens of 32/8 heads of 128 into an e4m3 pool, 259 MB, take 43.9 us (5.9
+// TB/s, 0.90 of the copy rate); the float64 rotation costs 2 us of it. Eight CTAs of four warps on an SM keep loads, turns and
 // stores of different tokens going side by side: four of eight warps take 46.8 us, and a CTA that takes several tokens
 // with the next one's loads under way more (63 us in registers, 97 us through shared memory): CTAs of one token are
 // dealt out as SMs come free.

@@ -17,12 +17,15 @@
 // the page numbers are fetched one tile further ahead. Rows are swizzled by 16-byte chunks so that the
 // fragment reads below meet no bank conflicts at 128-byte rows and wider.
 //
-// Measured: 131071 keys of 32/8 heads of 128 in F16, 537 MB, 99 us (5.4 TB/s, 0.83 of the copy rate; the SMs of some
+// Measured: 131071 keys of 32/8 heads of 128 in F16, 537 MB, 98 us (5.5 TB/s, 0.84 of the copy rate; the SMs of some
 // GPCs stream 12% slower than the others, and even shares wait for them); 64 requests over 2000 to 16000 e4m3 keys,
 // 901 MB, 175 us (5.1 TB/s, 0.78; the conversions' dependent chains with 8 warps on an SM - 12 warps with tiles of half
 // the size take an eighth more); 200 requests over 60 to 2048 keys of 14/2 heads of 64 in F16, 60 MB, 23 us (start, joins and
-// the second kernel are two thirds); one request over 1023 keys 8.4 us (two launches); 33 requests of 16 heads on one
-// F32 head, windows of 4096 keys, 80 MB, 42 us (the splitting of F32 operands).
+// the second kernel are two thirds); one request over 1023 keys 8.8 us (two launches); 33 requests of 16 heads on one
+// F32 head, windows of 4096 keys, 80 MB, 42 us (1009 instructions per tile of 8 keys; half of its 128 splits of
+// F32 operands are of q, the same ones for each tile). With 9 to 16 heads of 128 per KV head 255 registers do not hold q's halves and the
+// output: spills of 482 bytes a thread with e4m3, 142 with F16, 76 with F32 (36 with e4m3 and up to 8 heads). 64 requests over 2000 to
+// 16000 keys of 32/2 heads of 128: e4m3 225 MB, 158 us (1.4 TB/s), F16 450 MB, 105 us (4.3 TB/s); of 16/2 heads 53 and 83 us.
 //
 // Products. mma.sync tiles of 16 rows x 8 keys (scores) and 16 rows x 8 channels (values). With at most 8 query
 // heads per KV head the 16 rows are the heads' leading halves and, below them, their remainders: an F32
